@@ -43,8 +43,8 @@ int check(const nnrcu_kv_cache* c, const nnrcu_kv_attention_desc* d, bool buffer
 // 48 rows 32.1 and 32.6. 16 sequences of 8192 with 32 rows: 97 and 116.
 constexpr int kManyRows = 40;
 
-// How the work is divided: what runs at once on the SMs, or a block for each
-// quad of keys where those are fewer.
+// How the work is divided (one sequence at least): what runs at once on the SMs,
+// or a block for each quad of keys where those are fewer.
 void divide(const nnrcu_kv_cache& c, const nnrcu_kv_attention_desc& d, Args* p) {
   const long long rows = (long long)d.q_len * (d.q_heads / c.heads);
   // Many rows go to the kernel for blocks of 128, which has its products on
@@ -221,6 +221,8 @@ int nnrcu_kv_attention_workspace(const nnrcu_kv_cache* cache, const nnrcu_kv_att
   const int rc = check(cache, desc, false);
   if (rc != NNRCU_OK) return rc;
   if (!bytes) return set_error(NNRCU_ERR_INVALID, "bytes is NULL");
+  *bytes = 0;
+  if (desc->batch == 0) return NNRCU_OK;  // there are no rows to divide
   Args p{};
   divide(*cache, *desc, &p);
   *bytes = lay_out(*cache, *desc, &p, nullptr);
