@@ -622,8 +622,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
           top[n][e] = x * row_scale[n][e];
           grown |= top[n][e] > ref[n][e] + 8.f;
         }
-      // The largest r_j of a key that some row sees. One that is no number, in a
-      // tile with hidden keys, must not reach the rows that do not see its key.
+      // The largest r_j of a key that some row sees.
       float widest = 0.f;
 #pragma unroll
       for (int e = 0; e < C::kGroups; ++e)
@@ -631,7 +630,6 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
           const float x = fabsf(vs[lane * C::kGroups + e]);
           widest = x < INFINITY ? fmaxf(widest, x) : INFINITY;
         }
-      const bool strange = partial && __any_sync(~0u, widest == INFINITY);
       if (widest == INFINITY || (partial && (!((mask >> lane) & 1) || first + lane < any_lo || first + lane >= any_hi)))
         widest = 0.f;
       grown |= (__float_as_uint(widest) >> 23) > wide;
@@ -679,7 +677,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float w[4] = {s[i][n][0] * f0, s[i][n][1] * f0, s[i][n][2] * f1, s[i][n][3] * f1};
-            if (strange) {  // nothing of a hidden key
+            if (partial) {  // nothing of a hidden key, whatever its scale is
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (s[i][n][e] == 0.f) w[e] = 0.f;

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from nnr_b200 import ops
+from test_gpu_decode import TYPES, filled, generator, layout
 
 pytestmark = pytest.mark.gpu
 
@@ -21,3 +22,34 @@ def test_attention_of_an_empty_batch_behind_a_prefix():
     q = torch.zeros(1, 3, 4, 64, device="cuda", dtype=torch.bfloat16)
     y = ops.KVAttention(cache, 4).exec(q[:0], table[:0], lens[:0], prefix_table=table[0], prefix_len=20)
     assert y.shape == (0, 3, 4, 64) and y.dtype == torch.bfloat16
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind,batch,prefix,window", [((8, 0, 128, 2, 16), 2, 0, 60), ((4, 32, 128, 2, 16), 2, 0, 60),
+                                                      ((8, 0, 256, 1, 16), 2, 0, 60), ((8, 32, 96, 2, 16), 2, 0, 60),
+                                                      ((8, 0, 128, 2, 16), 40, 203, 150)])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("large", [1e6, 1e38])
+def test_attention_large_scales_of_unseen_values(kind, batch, prefix, window, zeros, large, t):
+    """Keys that lie in a tile with the window's first, or behind a sequence's
+    end, and are not seen: their values' scales do not matter however large they
+    are, not even where all that is seen is zero."""
+    cache = filled(kind, batch * 7 + 15, 5)
+    table, prefix_table = layout(cache, batch, 100, prefix, 4)
+    lens = torch.full((batch,), 90, dtype=torch.int32, device="cuda")
+    lens[1] = 33
+    seen = torch.zeros(cache.pages, 16, dtype=torch.bool, device="cuda")
+    for b in range(batch):
+        held = int(lens[b])
+        for at in range(max(0, prefix + held - 1 - window), prefix + held):
+            page = table[b, (at - prefix) // 16] if at >= prefix else prefix_table[at // 16]
+            seen[int(page), at % 16 if at < prefix else (at - prefix) % 16] = True
+    if zeros:
+        cache.v_scale.zero_()
+    q = torch.randn(batch, 2, 8, kind[2], generator=generator(4), device="cuda").to(TYPES[t])
+    op = ops.KVAttention(cache, 8, window=window)
+    want = op.exec(q, table, lens, max_len=100, prefix_table=prefix_table, prefix_len=prefix)
+    assert torch.isfinite(want).all() and bool((want == 0).all()) == zeros
+    cache.v_scale.copy_(torch.where(seen[:, None, :, None], cache.v_scale, large))
+    got = op.exec(q, table, lens, max_len=100, prefix_table=prefix_table, prefix_len=prefix)
+    assert torch.equal(got, want)
