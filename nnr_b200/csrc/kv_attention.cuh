@@ -190,10 +190,11 @@ __device__ __forceinline__ void locate(const Args& p, int unit_b, int head, int 
 }
 
 // The keys [lo, hi) of the unit's kind (own or prefix) that token i of a
-// sequence with len tokens of its own sees.
+// sequence with len tokens of its own sees. (Any window up to the largest int is
+// taken, and positions before 0 see nothing: the comparisons stay in range.)
 __device__ __forceinline__ void visible(const Args& p, bool own, int len, int i, int& lo, int& hi) {
   const int pos = p.prefix_len + len - p.q_len + i;
-  const int first = p.window ? max(0, pos - p.window + 1) : 0;
+  const int first = p.window && pos >= p.window ? pos - p.window + 1 : 0;
   lo = own ? max(0, first - p.prefix_len) : first;
   hi = own ? min(len, pos + 1 - p.prefix_len) : min(p.prefix_len, pos + 1);
 }
@@ -202,7 +203,7 @@ constexpr int kQuad = kWarps * kKeys;
 // Where the keys of a sequence's units start, a multiple of kKeys, and how
 // many quads they are (one at least, so that every row is written).
 __device__ __forceinline__ int first_key(const Args& p, bool own, int len) {
-  return own && p.window ? max(0, len - p.q_len - p.window + 1) / kKeys * kKeys : 0;
+  return own && p.window && len - p.q_len >= p.window ? (len - p.q_len - p.window + 1) / kKeys * kKeys : 0;
 }
 __device__ __forceinline__ int quads_of(const Args& p, bool own, int b) {
   const int len = own ? length_of(p, b) : p.prefix_len;

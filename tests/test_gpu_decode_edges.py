@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from nnr_b200 import ops
-from test_gpu_decode import TYPES, filled, generator, layout
+from test_gpu_decode import TYPES, attention_ref, filled, generator, layout, near
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +53,20 @@ def test_attention_large_scales_of_unseen_values(kind, batch, prefix, window, ze
     cache.v_scale.copy_(torch.where(seen[:, None, :, None], cache.v_scale, large))
     got = op.exec(q, table, lens, max_len=100, prefix_table=prefix_table, prefix_len=prefix)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("q_len,prefix", [(4, 0), (4, 40), (12, 40)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 3, 1 << 30])
+def test_attention_window_past_every_position(q_len, prefix, window, t):
+    """A window that hides nothing, on sequences with fewer tokens than queries too."""
+    kind = (8, 0, 64, 2, 16)
+    cache = filled(kind, 6 * 2 + 5, 1)
+    table, prefix_table = layout(cache, 6, 30, prefix, 2)
+    lens = torch.tensor([0, 1, 2, 3, 13, 30], dtype=torch.int32, device="cuda")
+    q = torch.randn(6, q_len, 8, 64, generator=generator(3), device="cuda").to(TYPES[t])
+    kw = dict(max_len=30, prefix_table=prefix_table, prefix_len=prefix)
+    want = ops.KVAttention(cache, 8).exec(q, table, lens, **kw)
+    ref, slack = attention_ref(cache, q, table, lens, prefix_table, prefix, 0, 64 ** -0.5, t)
+    near(want, ref, slack, t)
+    assert torch.equal(ops.KVAttention(cache, 8, window=window).exec(q, table, lens, **kw), want)
