@@ -341,7 +341,8 @@ int nnrcu_gap_f32_nhwc(const float* x, int n, int hw, int c, float* y, void* str
  * block_size is 32, 64, 128 or 256 (others: NNRCU_ERR_UNSUPPORTED). The
  * operands are host or device memory (whatever writes them on the device has
  * completed) and are laid out once, on the current device, into buffers that
- * the op owns; nnrcu_matmul_nbits_create returns when that is done.
+ * the op owns; nnrcu_matmul_nbits_create returns when that is done. A run on
+ * another current device is refused.
  * a is [m][k] with rows lda elements apart, y is [m][n] with rows ldy apart.
  * Made for the few rows of a decode step: any m works, but every 32 rows (16-bit
  * types) or 16 (fp32) read the codes again. */

@@ -603,6 +603,10 @@ int nnrcu_matmul_nbits_create(int k, int n, int block_size, int dtype, const uin
 int nnrcu_matmul_nbits_run(nnrcu_op* op, const void* a, int m, long long lda, void* y, long long ldy, void* stream) {
   if (!op || !a || !y) return set_error(NNRCU_ERR_INVALID, "NULL argument");
   if (op->kind != OP_MATMUL_NBITS) return set_error(NNRCU_ERR_INVALID, "not a MatMulNBits operator");
+  int device = 0;
+  NNRCU_CUDA(cudaGetDevice(&device));
+  if (device != op->device)
+    return set_error(NNRCU_ERR_INVALID, "the weights are on device %d, the current device is %d", op->device, device);
   if (m < 1 || (m > 1 && (lda < op->K || ldy < op->N)))
     return set_error(NNRCU_ERR_INVALID, "m = %d rows with strides %lld and %lld of k = %d and n = %d", m, lda, ldy,
                      op->K, op->N);

@@ -555,6 +555,7 @@ class MatMulNBits(Operator):
         if bias is not None and (bias.dtype != scales.dtype or tuple(bias.shape) != (n,)):
             raise ValueError(f"bias must be {scales.dtype} {(n,)}")
         self._plans = _Plans(self._plan)
+        self._device = torch.cuda.current_device()
         held = [None if t is None else t.contiguous() for t in (b, scales, zero_points, bias)]
         if any(t is not None and t.is_cuda for t in held):
             _on_current_device(*[t for t in held if t is not None and t.is_cuda])
@@ -580,7 +581,10 @@ class MatMulNBits(Operator):
     def exec(self, a: torch.Tensor, y: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """a [..., k], rows at any one distance, to y [..., n]."""
         shape, m, lda = self._plans((a.shape, a.stride(), a.dtype))
-        raw, context = _on_stream(stream, _on_current_device(a))
+        device = _on_current_device(a)
+        if device != self._device:
+            raise ValueError(f"the weights are on cuda:{self._device}, the current device is cuda:{device}")
+        raw, context = _on_stream(stream, device)
         y = _new(a, shape, context) if y is None else _given(y, shape, a)
         if m:
             rc = _nbits_run(self._op, a.data_ptr(), m, lda, y.data_ptr(), self.n, raw)

@@ -70,3 +70,14 @@ def test_attention_window_past_every_position(q_len, prefix, window, t):
     ref, slack = attention_ref(cache, q, table, lens, prefix_table, prefix, 0, 64 ** -0.5, t)
     near(want, ref, slack, t)
     assert torch.equal(ops.KVAttention(cache, 8, window=window).exec(q, table, lens, **kw), want)
+
+
+def test_matmul_nbits_refuses_another_device():
+    """Weights on another device than the current one are not read. (There is
+    one device here: the operator is told that its weights are elsewhere.)"""
+    op = ops.MatMulNBits(torch.zeros(8, 2, 16, dtype=torch.uint8), torch.ones(8, 2, dtype=torch.bfloat16), 64)
+    a = torch.zeros(2, 64, device="cuda", dtype=torch.bfloat16)
+    assert op.exec(a).shape == (2, 8)
+    op._device += 1
+    with pytest.raises(ValueError, match="weights are on cuda:1"):
+        op.exec(a)
