@@ -675,7 +675,8 @@ class KVCache:
 class KVAttention:
     """Causal attention of each sequence's newest tokens over a KVCache
     (nnrcu_kv_attention_run). scale: of the logits, 1 / sqrt(head_dim) by
-    default; window: how many positions up to its own a query sees, 0 for all."""
+    default; window: how many positions up to its own a query sees, 0 for all.
+    Both may be set anew between calls."""
 
     def __init__(self, cache: KVCache, q_heads: int, scale: Optional[float] = None, window: int = 0):
         if q_heads < 1 or q_heads % cache.heads:
@@ -685,7 +686,7 @@ class KVAttention:
         self._plans = _Plans(self._plan)
 
     def _plan(self, shape, strides, dtype, table_shape, table_strides, table_dtype, lens_shape, lens_strides, lens_dtype,
-              prefix_shape, prefix_strides, prefix_dtype, max_len, prefix_len):
+              prefix_shape, prefix_strides, prefix_dtype, max_len, prefix_len, window, scale):
         """(reference to the description, workspace bytes, the description itself)."""
         cache = self.cache
         if len(shape) != 4 or shape[2] != self.q_heads or shape[3] != cache.head_dim or shape[1] < 1:
@@ -706,8 +707,8 @@ class KVAttention:
                                  q_batch_stride=strides[0], q_token_stride=strides[1], q_head_stride=strides[2],
                                  table_pages=pages, table_stride=table_strides[0],
                                  max_len=pages * cache.page_size if max_len is None else max_len, prefix_len=prefix_len,
-                                 prefix_pages=0 if prefix_dtype is None else prefix_shape[0], window=self.window,
-                                 scale=self.scale)
+                                 prefix_pages=0 if prefix_dtype is None else prefix_shape[0], window=window,
+                                 scale=scale)
         need = C.c_size_t()
         call("nnrcu_kv_attention_workspace", cache._desc, C.byref(d), C.byref(need))
         return C.byref(d), need.value, d
@@ -727,10 +728,11 @@ class KVAttention:
                lens.stride(), lens.dtype)
         if prefix_table is None:
             prefix = None
-            key += (None, None, None, max_len, prefix_len)
+            key += (None, None, None, max_len, prefix_len, self.window, self.scale)
         else:
             prefix = prefix_table.data_ptr()
-            key += (prefix_table.shape, prefix_table.stride(), prefix_table.dtype, max_len, prefix_len)
+            key += (prefix_table.shape, prefix_table.stride(), prefix_table.dtype, max_len, prefix_len, self.window,
+                    self.scale)
         ref, need, _ = self._plans(key)
         device = _on_current_device(q, page_table, lens, cache.k)
         if prefix_table is not None:

@@ -81,3 +81,19 @@ def test_matmul_nbits_refuses_another_device():
     op._device += 1
     with pytest.raises(ValueError, match="weights are on cuda:1"):
         op.exec(a)
+
+
+def test_attention_takes_a_scale_and_a_window_set_anew():
+    cache = filled((8, 0, 64, 1, 16), 9, 1)
+    table, _ = layout(cache, 2, 60, 0, 1)
+    lens = torch.tensor([60, 41], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 1, 2, 64, generator=generator(2), device="cuda").bfloat16()
+    op = ops.KVAttention(cache, 2)
+    seen = [op.exec(q, table, lens)]
+    for kw in (dict(scale=1.0), dict(scale=-0.5, window=7), dict(window=3), dict()):
+        op.scale, op.window = kw.get("scale", 64 ** -0.5), kw.get("window", 0)
+        y = op.exec(q, table, lens)
+        assert torch.equal(y, ops.KVAttention(cache, 2, **kw).exec(q, table, lens))
+        seen.append(y)
+    assert torch.equal(seen[0], seen[4])
+    assert all(not torch.equal(seen[i], seen[j]) for i in range(4) for j in range(i))
