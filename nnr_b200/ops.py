@@ -466,6 +466,14 @@ def _dtype_code(dtype: torch.dtype) -> int:
     return code
 
 
+def _c_int(**numbers) -> dict:
+    """The numbers, for a C int each (ctypes would drop the bits that it has not)."""
+    for name, n in numbers.items():
+        if not -1 << 31 <= n < 1 << 31:
+            raise ValueError(f"{name} must fit 32 bits, got {n}")
+    return numbers
+
+
 def _on_current_device(*tensors: torch.Tensor) -> int:
     """Index of the current device, on which every tensor has to be."""
     at = torch.cuda.current_device()
@@ -545,6 +553,7 @@ class MatMulNBits(Operator):
         n, groups, block = b.shape[0], b.shape[1], 2 * b.shape[2]
         self.n, self.k, self.block_size, self.dtype = n, int(k), block, scales.dtype
         code = _dtype_code(scales.dtype)
+        _c_int(n=n, k=self.k)
         if n < 1 or block < 1 or groups != -(-self.k // block):
             raise ValueError(f"b {tuple(b.shape)} does not hold k = {k} in blocks of {block}")
         if tuple(scales.shape) != (n, groups):
@@ -571,6 +580,7 @@ class MatMulNBits(Operator):
             raise ValueError(f"A must be [..., {self.k}], got {tuple(shape)}")
         lead = [(n, s) for n, s in zip(shape[:-1], strides[:-1]) if n != 1]
         m = int(np.prod(shape[:-1], dtype=np.int64))
+        _c_int(rows=m)
         lda = lead[-1][1] if lead else self.k
         if m and any(s != n2 * s2 for (_, s), (n2, s2) in zip(lead, lead[1:])):
             raise ValueError("A's leading dims must have one stride")
@@ -610,8 +620,8 @@ class KVCache:
                  buffers=None):
         self.pages, self.page_size, self.heads, self.head_dim = int(pages), int(page_size), int(heads), int(head_dim)
         self.bits, self.group = int(bits), int(group) or int(head_dim)
-        self.desc = _lib.KvCacheDesc(pages=self.pages, page_size=self.page_size, heads=self.heads,
-                                     head_dim=self.head_dim, bits=self.bits, group=self.group)
+        self.desc = _lib.KvCacheDesc(**_c_int(pages=self.pages, page_size=self.page_size, heads=self.heads,
+                                              head_dim=self.head_dim, bits=self.bits, group=self.group))
         code_bytes, scale_bytes = C.c_size_t(), C.c_size_t()
         call("nnrcu_kv_cache_sizes", C.byref(self.desc), C.byref(code_bytes), C.byref(scale_bytes))
         rows = (self.pages, self.heads, self.page_size)
@@ -703,12 +713,11 @@ class KVAttention:
                                          or (prefix_shape[0] > 1 and prefix_strides[0] != 1)):
             raise ValueError("prefix_table must be a contiguous int32 [pages]")
         pages = table_shape[1]
-        d = _lib.KvAttentionDesc(batch=batch, q_len=shape[1], q_heads=self.q_heads, dtype=_dtype_code(dtype),
-                                 q_batch_stride=strides[0], q_token_stride=strides[1], q_head_stride=strides[2],
-                                 table_pages=pages, table_stride=table_strides[0],
-                                 max_len=pages * cache.page_size if max_len is None else max_len, prefix_len=prefix_len,
-                                 prefix_pages=0 if prefix_dtype is None else prefix_shape[0], window=window,
-                                 scale=scale)
+        ints = _c_int(batch=batch, q_len=shape[1], q_heads=self.q_heads, dtype=_dtype_code(dtype), table_pages=pages,
+                      max_len=pages * cache.page_size if max_len is None else max_len, prefix_len=prefix_len,
+                      prefix_pages=0 if prefix_dtype is None else prefix_shape[0], window=window)
+        d = _lib.KvAttentionDesc(**ints, q_batch_stride=strides[0], q_token_stride=strides[1], q_head_stride=strides[2],
+                                 table_stride=table_strides[0], scale=scale)
         need = C.c_size_t()
         call("nnrcu_kv_attention_workspace", cache._desc, C.byref(d), C.byref(need))
         return C.byref(d), need.value, d

@@ -97,3 +97,27 @@ def test_attention_takes_a_scale_and_a_window_set_anew():
         seen.append(y)
     assert torch.equal(seen[0], seen[4])
     assert all(not torch.equal(seen[i], seen[j]) for i in range(4) for j in range(i))
+
+
+def test_numbers_past_32_bits_are_refused():
+    """Not answered as what is left of them in 32 bits."""
+    cache = filled((8, 0, 64, 2, 16), 9, 1)
+    table, prefix_table = layout(cache, 2, 60, 16, 1)
+    lens = torch.tensor([60, 41], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 1, 4, 64, generator=generator(2), device="cuda").bfloat16()
+    op = ops.KVAttention(cache, 4)
+    kw = dict(max_len=60, prefix_table=prefix_table, prefix_len=16)
+    for bad in (dict(max_len=2 ** 32 + 60), dict(prefix_len=2 ** 32 + 16), dict(prefix_len=-2 ** 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            op.exec(q, table, lens, **{**kw, **bad})
+    op.window = 2 ** 32 + 5
+    with pytest.raises(ValueError, match="32 bits"):
+        op.exec(q, table, lens, **kw)
+    for bad in (dict(pages=2 ** 32 + 9), dict(heads=2 ** 32 + 2), dict(group=2 ** 32)):
+        with pytest.raises(ValueError, match="32 bits"):
+            ops.KVCache(**{**dict(pages=9, page_size=16, heads=2, head_dim=64), **bad},
+                        buffers={n: getattr(cache, n) for n in ("k", "k_scale", "v", "v_scale")})
+    linear = ops.MatMulNBits(torch.zeros(1, 1, 16, dtype=torch.uint8), torch.ones(1, 1, dtype=torch.half), 1)
+    a = torch.empty(2 ** 32 + 5, 1, dtype=torch.half, device="cuda")
+    with pytest.raises(ValueError, match="32 bits"):
+        linear.exec(a)
