@@ -515,7 +515,7 @@ int launch(const NbitsArgs& p, cudaStream_t st) {
     NNRCU_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
     ready.fetch_or(1ull << device, std::memory_order_relaxed);
   }
-  const int blocks = (p.m + C::kRows - 1) / C::kRows, items = (p.n + C::kOuts - 1) / C::kOuts;
+  const int blocks = (int)(((long long)p.m + C::kRows - 1) / C::kRows), items = (p.n + C::kOuts - 1) / C::kOuts;
   for (int y0 = 0; y0 < blocks; y0 += 65535) {  // what a grid holds
     NbitsArgs q = p;
     const long long skip = (long long)y0 * C::kRows;

@@ -121,3 +121,14 @@ def test_numbers_past_32_bits_are_refused():
     a = torch.empty(2 ** 32 + 5, 1, dtype=torch.half, device="cuda")
     with pytest.raises(ValueError, match="32 bits"):
         linear.exec(a)
+
+
+def test_matmul_nbits_of_the_most_rows():
+    """2^31 - 1 rows, which pass 2^31 when they are rounded up to a block's."""
+    op = ops.MatMulNBits(torch.full((1, 1, 16), 0x99, dtype=torch.uint8), torch.ones(1, 1, dtype=torch.half), 1)
+    a = torch.empty(2 ** 31 - 1, 1, dtype=torch.half, device="cuda").uniform_(-1, 1, generator=generator(1))
+    y = torch.full_like(a, float("nan"))
+    op.exec(a, y=y)
+    assert torch.equal(y, a)  # a weight of 9 - 8 times 1
+    del a, y
+    torch.cuda.empty_cache()
