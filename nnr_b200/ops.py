@@ -507,6 +507,17 @@ def _given(y: torch.Tensor, shape, like: torch.Tensor) -> torch.Tensor:
     return y
 
 
+class _Fixed:
+    """An object whose attributes named in _fixed are set once: descriptions,
+    plans and addresses that its calls use were made from them."""
+    _fixed = frozenset()
+
+    def __setattr__(self, name, value):
+        if name in self._fixed and name in self.__dict__:
+            raise AttributeError(f"{name} is fixed once the {type(self).__name__} is made")
+        super().__setattr__(name, value)
+
+
 class _Plans:
     """What an operator has checked and worked out for calls with given sizes,
     strides and types: the answer to make(*key), for the last keys seen."""
@@ -530,7 +541,7 @@ _cache_read = lib.nnrcu_kv_cache_read
 _attention_run = lib.nnrcu_kv_attention_run
 
 
-class MatMulNBits(Operator):
+class MatMulNBits(_Fixed, Operator):
     """MatMulNBits: Y = A x W^T + bias with 4-bit W [n, k] that has a scale, and
     where given a zero point, for each block of block_size consecutive k:
     W[n, i] = (q[n, i] - z[n, i // block_size]) * scales[n, i // block_size].
@@ -544,6 +555,7 @@ class MatMulNBits(Operator):
     out once on the current device and not needed afterwards.
     """
     op_type = "MatMulNBits"
+    _fixed = frozenset(("n", "k", "block_size", "dtype"))
 
     def __init__(self, b: torch.Tensor, scales: torch.Tensor, k: int, zero_points: Optional[torch.Tensor] = None,
                  bias: Optional[torch.Tensor] = None):
@@ -603,7 +615,7 @@ class MatMulNBits(Operator):
         return y
 
 
-class KVCache:
+class KVCache(_Fixed):
     """A paged key/value cache in 8 or 4 bits (nnrcu_kv_cache): the codes and
     scales of every token and head, in pages of page_size tokens. A token's
     slot is page * page_size + its row in the page; which pages a sequence has
@@ -614,7 +626,9 @@ class KVCache:
     or 7; it stands for q * scale. buffers: existing tensors k, k_scale, v,
     v_scale (codes int8, or uint8 with two 4-bit codes a byte, even channels
     in the low nibble and 8 added; scales fp32) instead of zeroed new ones.
+    They may be written to, but not replaced.
     """
+    _fixed = frozenset(("pages", "page_size", "heads", "head_dim", "bits", "group", "desc", "k", "k_scale", "v", "v_scale"))
 
     def __init__(self, pages: int, page_size: int, heads: int, head_dim: int, bits: int = 8, group: int = 0,
                  buffers=None):
@@ -682,11 +696,12 @@ class KVCache:
         return k, v
 
 
-class KVAttention:
+class KVAttention(_Fixed):
     """Causal attention of each sequence's newest tokens over a KVCache
     (nnrcu_kv_attention_run). scale: of the logits, 1 / sqrt(head_dim) by
     default; window: how many positions up to its own a query sees, 0 for all.
     Both may be set anew between calls."""
+    _fixed = frozenset(("cache", "q_heads"))
 
     def __init__(self, cache: KVCache, q_heads: int, scale: Optional[float] = None, window: int = 0):
         if q_heads < 1 or q_heads % cache.heads:

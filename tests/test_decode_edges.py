@@ -5,6 +5,8 @@ from pathlib import Path
 
 import pytest
 
+from nnr_b200 import ops
+
 ROOT = Path(__file__).resolve().parent.parent
 
 EMPTY = """
@@ -28,3 +30,18 @@ def test_an_empty_batch_needs_no_workspace(dim, prefix):
     r = subprocess.run([sys.executable, "-c", EMPTY.format(dim=dim, prefix=prefix)], cwd=ROOT, capture_output=True,
                        text=True)
     assert r.returncode == 0, (r.returncode, r.stderr)
+
+
+@pytest.mark.parametrize("kind,names", [
+    (ops.MatMulNBits, ("n", "k", "block_size", "dtype")),
+    (ops.KVCache, ("pages", "page_size", "heads", "head_dim", "bits", "group", "desc", "k", "k_scale", "v", "v_scale")),
+    (ops.KVAttention, ("cache", "q_heads"))])
+def test_what_calls_rely_on_is_set_once(kind, names):
+    """Descriptions hold sizes and addresses: a cache whose k is replaced would
+    write to the old one's freed memory."""
+    x = kind.__new__(kind)
+    for name in names:
+        setattr(x, name, 1)
+        with pytest.raises(AttributeError, match=name):
+            setattr(x, name, 2)
+        assert getattr(x, name) == 1
