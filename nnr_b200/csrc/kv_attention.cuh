@@ -84,9 +84,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Operands are fp16: codes are exact in it, q and the weights p_j r_j are
-// scaled by a power of two for each row of q and for each warp to lie below
-// 2^15, where fp16 has 11 bits down to 2^-29 of that and steps of 2^-39 below.
+// Operands are fp16: codes are exact in it; q is scaled by a power of two for
+// each row to lie below 2^15, where fp16 has 11 bits down to 2^-29 of that and
+// steps of 2^-39 below. So are the weights p_j r_j, by a unit of each row's that
+// puts the largest so far at 2^6 or more: a weight keeps 11 bits down to 2^-20
+// of the largest weight, whatever larger values the row all but leaves out.
 // PARTS = 2 (fp32 tensors) holds a value as the sum of two of them (22 bits).
 template <int PARTS>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[PARTS]) {
@@ -100,6 +102,18 @@ __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[PAR
     }
   }
 }
+
+// A row's unit is 2^(e - 127), e from 6 to 245; its weights stay below 2^15.
+constexpr int kFirstUnit = 245;
+// The unit that puts a largest weight m at 2^6 or more (as far as the range
+// goes); `before` is the unit in which the earlier weights' largest is there.
+__device__ __forceinline__ int unit_for(float m, int before) {
+  return 260 - min(max(max((int)(__float_as_uint(m) >> 23), 260 - before), 260 - kFirstUnit), 254);
+}
+// 2^-n for n from 0 on, 0 past fp32's range.
+__device__ __forceinline__ float shrink_by(int n) { return n > 126 ? 0.f : __uint_as_float((127 - n) << 23); }
+// By how many powers of two what is relative to ref shrinks when that rises to next.
+__device__ __forceinline__ int rise_of(float ref, float next) { return next == -INFINITY ? 0 : (int)fminf(next - ref, 400.f); }
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t b0, const uint32_t b1) {
   asm volatile(
@@ -357,16 +371,15 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
       }
     }
     __syncthreads();
-    // What this lane's rows 8 n + 2 t + e see, and what all and any do.
-    int lo[NT][2], hi[NT][2], all_lo = 0, all_hi = 1 << 30, any_lo = 1 << 30, any_hi = 0;
+    // What all of this lane's rows 8 n + 2 t + e see, and any does.
+    int all_lo = 0, all_hi = 1 << 30, any_lo = 1 << 30, any_hi = 0;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        lo[n][e] = row_lo[8 * n + 2 * t + e], hi[n][e] = row_hi[8 * n + 2 * t + e];
-        if (row_y[8 * n + 2 * t + e] >= 0 && hi[n][e] > lo[n][e])
-          any_lo = min(any_lo, lo[n][e]), any_hi = max(any_hi, hi[n][e]);
-        all_lo = max(all_lo, lo[n][e]), all_hi = min(all_hi, hi[n][e]);
+        const int lo = row_lo[8 * n + 2 * t + e], hi = row_hi[8 * n + 2 * t + e];
+        if (row_y[8 * n + 2 * t + e] >= 0 && hi > lo) any_lo = min(any_lo, lo), any_hi = max(any_hi, hi);
+        all_lo = max(all_lo, lo), all_hi = min(all_hi, hi);
       }
     any_lo = __reduce_min_sync(~0u, any_lo);
     any_hi = __reduce_max_sync(~0u, any_hi);
@@ -511,11 +524,15 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
     for (int i = 0; i < kTiles; ++i)
 #pragma unroll
       for (int n = 0; n < NT; ++n) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
-    // ref: what the weights are relative to, a logit within 2^8 of the largest
+    // ref: what p is relative to, a whole number at most 6 below the largest
+    // logit; unit: of the weights p r and of o
     float ref[NT][2], l[NT][2];
+    int unit[NT][2];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) ref[n][0] = ref[n][1] = -INFINITY, l[n][0] = l[n][1] = 0.f;
-    uint32_t wide = 15;  // weights are held times 2^(6 - (wide - 127)), wide the exponent of the largest r_j so far
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) ref[n][e] = -INFINITY, l[n][e] = 0.f, unit[n][e] = kFirstUnit;
+    float most_unit = 0.f;  // the largest of the warp's rows that have seen a key
 
     int slot = 0;  // of this tile's keys; its values are in the next one
     for (int n_tile = 0; n_tile < my_tiles; ++n_tile) {
@@ -591,15 +608,19 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
       const bool partial = mask != ~0u || first < all_lo || first + kKeys > all_hi;
       if (partial) {
 #pragma unroll
-        for (int i = 0; i < kKeys / 16; ++i)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int f = 0; f < 2; ++f) {
+            const int lo = row_lo[8 * n + 2 * t + f], hi = row_hi[8 * n + 2 * t + f];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int in = i * 16 + 8 * (e >> 1) + g, at = first + in;
-              const bool hidden = (((mask >> in) & 1) == 0) | (at < lo[n][e & 1]) | (at >= hi[n][e & 1]);
-              s[i][n][e] = hidden ? -INFINITY : s[i][n][e];
-            }
+            for (int i = 0; i < kKeys / 16; ++i)
+#pragma unroll
+              for (int e = f; e < 4; e += 2) {
+                const int in = i * 16 + 8 * (e >> 1) + g, at = first + in;
+                const bool hidden = (((mask >> in) & 1) == 0) | (at < lo) | (at >= hi);
+                s[i][n][e] = hidden ? -INFINITY : s[i][n][e];
+              }
+          }
       }
 
       // The values have come; the next ones take the keys' slot.
@@ -609,8 +630,9 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
       __syncwarp();
       slot = slot_next;
 
-      // Running softmax. What the weights are relative to moves only when a
-      // logit passes it by 2^8: they stay below 2^8, and o is seldom rescaled.
+      // Running softmax. What p is relative to moves only when a logit passes it
+      // by 2^6: p stays below that, and o is seldom rescaled. Nor does the unit
+      // move before some r_j could take a weight past 2^15.
       bool grown = false;
       float top[NT][2];
 #pragma unroll
@@ -621,23 +643,19 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
 #pragma unroll
           for (int i = 1; i < kKeys / 16; ++i) x = fmaxf(x, fmaxf(s[i][n][e], s[i][n][2 + e]));
           top[n][e] = x * row_scale[n][e];
-          grown |= top[n][e] > ref[n][e] + 8.f;
+          grown |= top[n][e] > ref[n][e] + 6.f;
         }
-      // The largest r_j of a key that some row sees.
-      float widest = 0.f;
+      // The largest r_j of key j.
+      auto largest = [&](int key) {
+        float x = 0.f;
 #pragma unroll
-      for (int e = 0; e < C::kGroups; ++e)
-        if (e == 0 || e < groups) {
-          const float x = fabsf(vs[lane * C::kGroups + e]);
-          widest = x < INFINITY ? fmaxf(widest, x) : INFINITY;
-        }
-      if (widest == INFINITY || (partial && (!((mask >> lane) & 1) || first + lane < any_lo || first + lane >= any_hi)))
-        widest = 0.f;
-      grown |= (__float_as_uint(widest) >> 23) > wide;
-      if (__any_sync(~0u, grown)) {
-        const uint32_t now = max(wide, __reduce_max_sync(~0u, __float_as_uint(widest) >> 23));
-        const float shrink = now - wide > 126 ? 0.f : __uint_as_float((127 - (now - wide)) << 23);
-        wide = now;
+        for (int e = 0; e < C::kGroups; ++e)
+          if (e == 0 || e < groups) x = fmaxf(x, fabsf(vs[key * C::kGroups + e]));
+        return x;
+      };
+      grown |= largest(lane) * most_unit >= 0x1p9f;
+      const bool moves = __any_sync(~0u, grown);
+      if (moves) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -646,16 +664,14 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
             x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
             x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
             x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
-            x = fmaxf(x, ref[n][e]);
-            const float keep = x == -INFINITY ? 1.f : exp2_fast(ref[n][e] - x);
+            x = fmaxf(ceilf(x), ref[n][e]);
+            const int rise = rise_of(ref[n][e], x);
             ref[n][e] = x;
-            l[n][e] *= keep;
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i) o[i][n][e] *= keep * shrink, o[i][n][2 + e] *= keep * shrink;
+            l[n][e] *= shrink_by(rise);
+            unit[n][e] += rise;  // what o, as it stands, is in now
           }
       }
       __syncwarp();
-      const float per_unit = __uint_as_float((260 - wide) << 23);  // 2^(6 - (wide - 127))
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const float r0 = ref[n][0] == -INFINITY ? 0.f : ref[n][0], r1 = ref[n][1] == -INFINITY ? 0.f : ref[n][1];
@@ -667,14 +683,44 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
             l[n][e & 1] += s[i][n][e];
           }
       }
+      if (moves) {
+        float r[kKeys / 16][2];
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i) r[i][0] = largest(i * 16 + g), r[i][1] = largest(i * 16 + 8 + g);
+        most_unit = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = 0.f;
+#pragma unroll
+            for (int i = 0; i < kKeys / 16; ++i) x = fmaxf(x, fmaxf(s[i][n][e] * r[i][0], s[i][n][2 + e] * r[i][1]));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+            const int next = unit_for(x, unit[n][e]);
+            const float by = shrink_by(unit[n][e] - next);
+            unit[n][e] = next;
+            if (ref[n][e] > -INFINITY) most_unit = fmaxf(most_unit, __uint_as_float(next << 23));
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) o[i][n][e] *= by, o[i][n][2 + e] *= by;
+          }
+        most_unit = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(most_unit)));
+      }
+      __syncwarp();
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < kKeys / 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][n][e] *= __uint_as_float(unit[n][e & 1] << 23);
 
       // o += D^T (p r)^T
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i) {
         uint32_t b[NT][PARTS][2];
         auto weights = [&](int grp) {
-          const float f0 = vs[(i * 16 + g) * C::kGroups + grp] * per_unit;
-          const float f1 = vs[(i * 16 + 8 + g) * C::kGroups + grp] * per_unit;
+          const float f0 = vs[(i * 16 + g) * C::kGroups + grp], f1 = vs[(i * 16 + 8 + g) * C::kGroups + grp];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float w[4] = {s[i][n][0] * f0, s[i][n][1] * f0, s[i][n][2] * f1, s[i][n][3] * f1};
@@ -724,7 +770,6 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
     // chunk (8 bits), 4 g + 2 st, + 1 of a chunk's half st (4 bits).
     __syncthreads();
     float* const mo = reinterpret_cast<float*>(smem) + warp * C::kRows * C::kMergeRow;
-    const float real = __uint_as_float((wide - 6) << 23);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -734,6 +779,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
         x += __shfl_xor_sync(~0u, x, 8);
         x += __shfl_xor_sync(~0u, x, 16);
         const int r = 8 * n + 2 * t + e;
+        const float real = __uint_as_float((254 - unit[n][e]) << 23);
         if (g == 0) warp_ml[warp][r] = make_float2(ref[n][e], x);
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {

@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
   volatile int* const abort_flag = words + 1;
   float* const scales = reinterpret_cast<float*>(smem + L::kScales);
   uint32_t* const masks = reinterpret_cast<uint32_t*>(smem + L::kMasks);
-  uint32_t* const widests = reinterpret_cast<uint32_t*>(smem + L::kWidest);
+  float* const widests = reinterpret_cast<float*>(smem + L::kWidest);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   pdl_launch();
@@ -230,7 +230,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
       }
       float ref = -INFINITY;
       float2 l = make_float2(0.f, 0.f), l2 = make_float2(0.f, 0.f);
-      uint32_t wide = 15;
+      int unit = kFirstUnit;
+      float room = 268.f - kFirstUnit;  // what p's and r's exponents may be together for a weight to stay below 2^15
       for (int n = 0; n < tiles && ok; ++n) {
         const int g = done + n, buf = g & 1, slot = g % kRing;
         const int first = begin + n * kN;
@@ -290,35 +291,50 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
         top = fmaxf(top, other(top, ok));
         if (!ok) break;
         // the exponent of the largest value scale of a key that some row sees
-        const uint4 four = *reinterpret_cast<const uint4*>(widests + slot * 4);
-        const uint32_t widest = max(max(four.x, four.y), max(four.z, four.w));
-        const bool grown = __any_sync(~0u, top > ref + 8.f || widest > wide);
+        const float4 four = *reinterpret_cast<const float4*>(widests + slot * 4);
+        const float widest = fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w));
+        // p passes 2^8, or a weight may pass 2^15: p is at most 2^(top - ref)
+        const float above = top - ref;
+        const bool moves = __any_sync(~0u, above > 8.f || above + widest > room);
         ok = __all_sync(~0u, n == 0 || wait(O_DONE, g - 1));  // the last tile's weights are used, and O holds it
         if (!ok) break;
-        if (grown) {  // the same in both halves
-          const uint32_t now = max(wide, widest);
-          const float shrink = now - wide > 126 ? 0.f : __uint_as_float((127 - (now - wide)) << 23);
-          wide = now;
-          const float next = fmaxf(top, ref);
-          const float keep = next == -INFINITY ? 1.f : exp2_fast(ref - next);
+        const float2 factor = make_float2(row_scale, row_scale);
+        if (moves) {  // the same in both halves
+          const float next = fmaxf(ceilf(top), ref);
+          const int rise = rise_of(ref, next);
+          const float keep = shrink_by(rise), base = next == -INFINITY ? 0.f : next;
           ref = next;
           l.x *= keep, l.y *= keep, l2.x *= keep, l2.y *= keep;
-          if (n > 0) {
+          unit += rise;  // what O, as it stands, is in now
+          float m[2] = {0.f, 0.f};  // the tile's largest weight
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 r = *reinterpret_cast<const float2*>(vs + 64 * half + 32 * c + 2 * j);
+              const float2 q = __ffma2_rn(x[c][j], factor, make_float2(-base, -base));
+              m[0] = fmaxf(m[0], exp2_fast(q.x) * fabsf(r.x)), m[1] = fmaxf(m[1], exp2_fast(q.y) * fabsf(r.y));
+            }
+          float most_weight = fmaxf(m[0], m[1]);
+          most_weight = fmaxf(most_weight, other(most_weight, ok));
+          if (!ok) break;
+          const int fit = unit_for(most_weight, unit), by = unit - fit;
+          unit = fit, room = 268.f - (float)fit;
+          if (n > 0 && __any_sync(~0u, by != 0)) {
+            const float f = shrink_by(by);
             ptx::tc_fence_after();
 #pragma unroll 1
             for (int i = half * (DIM / 64); i < (half + 1) * (DIM / 64); ++i) {
               uint32_t o[32];
               ptx::tmem_ld32(t_o + lanes + 32 * i, o);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * (keep * shrink));
+              for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
               tmem_st32(t_o + lanes + 32 * i, o);
             }
           }
         }
-        const float base = ref == -INFINITY ? 0.f : ref;
-        const float2 minus = make_float2(-base, -base), factor = make_float2(row_scale, row_scale);
-        const float unit = __uint_as_float((260 - wide) << 23);
-        const float2 per_unit = make_float2(unit, unit);
+        const float base = ref == -INFINITY ? 0.f : ref, times = __uint_as_float(unit << 23);
+        const float2 minus = make_float2(-base, -base), per_unit = make_float2(times, times);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
@@ -329,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
               float2 q = __ffma2_rn(x[c][j + e], factor, minus);
               q = make_float2(exp2_fast(q.x), exp2_fast(q.y));
               (j & 2 ? l2 : l) = __fadd2_rn(j & 2 ? l2 : l, q);
-              x[c][j + e] = __fmul2_rn(q, __fmul2_rn(e ? make_float2(f.z, f.w) : make_float2(f.x, f.y), per_unit));
+              x[c][j + e] = __fmul2_rn(__fmul2_rn(q, per_unit), e ? make_float2(f.z, f.w) : make_float2(f.x, f.y));
             }
           }
           if (partial) {  // nothing of a hidden key, whatever its scale is
@@ -367,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
       ptx::tc_fence_after();
       const bool whole = n_quads == at.quads && !p.prefix_len;
       const long long segment = ((own ? (long long)at.b * w.units : 0) + at.unit + blockIdx.x) * kM + r;
-      const float real = tiles > 0 && ok && sum != 0.f ? __uint_as_float((wide - 6) << 23) : 0.f;
+      const float real = tiles > 0 && ok && sum != 0.f ? __uint_as_float((254 - unit) << 23) : 0.f;
       const float f = whole && real != 0.f ? real / sum : real;
       // O by 32 channels through shared memory (every product has ended), so
       // that a store is one row's 32 and not one channel of 32 rows.
@@ -483,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
         const uint32_t r_bits = __float_as_uint(scales[(kRing + slot) * kN + key]) & 0x7FFFFFFFu;
         const bool counts = j >= any_lo && j < any_hi && r_bits < 0x7F800000u;  // a hidden key's is 0
         const uint32_t widest = __reduce_max_sync(~0u, counts ? r_bits >> 23 : 0u);
-        if (lane == 0) widests[slot * 4 + warp - 8] = widest;
+        if (lane == 0) widests[slot * 4 + warp - 8] = (float)widest;
         convert(raw_mine + (n & 1) * 2 * L::kCodes, smem + L::kK);
         ptx::fence_proxy_async_smem();
         ptx::mbar_arrive(bars + K_FULL);

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from nnr_b200 import ops
-from test_gpu_decode import TYPES, attention_ref, filled, generator, layout, near
+from test_gpu_decode import HALF, TYPES, attention_ref, filled, generator, layout, near, values
 
 pytestmark = pytest.mark.gpu
 
@@ -132,3 +132,88 @@ def test_matmul_nbits_of_the_most_rows():
     assert torch.equal(y, a)  # a weight of 9 - 8 times 1
     del a, y
     torch.cuda.empty_cache()
+
+
+def near_by_weight(got, cache, q, table, lens, prefix_table, prefix, scale, t):
+    """As test_gpu_decode.near for one query a sequence, but what a weight p_j r_j
+    loses (its fp16 steps of 2^-24, half of one, in units in which the row's
+    largest weight is at least 2^6: 2^-31 of that) is counted against the largest
+    weight and not against the largest value. (Twice, since the largest code of
+    that key may be less than the type's.)"""
+    batch, _, q_heads, dim = q.shape
+    k, v = (values(cache, p) for p in "kv")
+    for b in range(batch):
+        rows = [torch.cat((x[prefix_table.long()].flatten(0, 1)[:prefix], x[table[b].long()].flatten(0, 1)[:int(lens[b])]))
+                for x in (k, v)]
+        kk, vv = (r.repeat_interleave(q_heads // cache.heads, 1).transpose(0, 1) for r in rows)
+        qq = q[b, 0].double()[:, :, None] * scale
+        x = (kk @ qq)[..., 0]
+        p = torch.softmax(x, -1)
+        want = (p[:, None] @ vv)[:, 0]
+        n, terms = p.shape[1], (kk.abs() @ qq.abs())[..., 0].amax(-1, keepdim=True)
+        loose = HALF[t] + 2 * (dim / 16 + 16) * 2.0 ** -23 * terms + 2.0 ** -20 + (n / 16 + 64) * 2.0 ** -23
+        slack = loose * (p[:, None] @ vv.abs())[:, 0]
+        slack += n * 2.0 ** -31 * (p * vv.abs().amax(-1)).amax(-1, keepdim=True) * 2
+        near(got[b, 0], want, slack, t)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind,batch,longest,prefix", [
+    ((8, 0, 64, 1, 16), 2, 120, 0), ((8, 0, 64, 1, 16), 40, 40, 200), ((4, 32, 128, 1, 16), 2, 300, 0),
+    ((8, 0, 256, 1, 16), 2, 300, 0), ((8, 0, 128, 1, 16), 1, 9000, 0), ((8, 0, 128, 4, 16), 40, 20, 12000),
+    ((4, 0, 64, 4, 16), 40, 20, 12000)])
+@pytest.mark.parametrize("power", [0, 16, 24, 40])
+def test_attention_large_values_that_weigh_next_to_nothing(kind, batch, longest, prefix, power, t):
+    """Keys whose values are 2^power times the others', and which no query gives
+    a weight of 2^-60: the others keep their precision."""
+    bits, group, dim, heads, page = kind
+    per, shared = -(-longest // page), -(-prefix // page)
+    cache = filled(kind, batch * per + shared, 3)
+    pages = torch.arange(cache.pages, dtype=torch.int32, device="cuda")
+    prefix_table, table = pages[:shared].contiguous(), pages[shared:].view(batch, per)
+    q = torch.randn(batch, 1, heads * 4, dim, generator=generator(9), device="cuda").to(TYPES[t])
+    q[..., 0] = 16
+    for page_of in ([table[b, i] for b in range(batch) for i in (0, per // 2)] if longest >= 40 else
+                    [prefix_table[i] for i in (0, 2, shared // 2, shared - 2)]):
+        at = (int(page_of), slice(None), 7)
+        # a code of -127 (-7) in channel 0, where every query is 16, and zeros elsewhere
+        cache.k[at] = 0 if bits == 8 else 0x88
+        cache.k[at[0], :, 7, 0] = -127 if bits == 8 else 0x81
+        cache.k_scale[at] = 60 * dim ** 0.5 / (16 * (127 if bits == 8 else 7))  # a logit of -60
+        cache.v_scale[at] *= 2.0 ** power
+    lens = torch.full((batch,), longest, dtype=torch.int32, device="cuda")
+    got = ops.KVAttention(cache, heads * 4).exec(q, table, lens, prefix_table=prefix_table, prefix_len=prefix)
+    near_by_weight(got, cache, q, table, lens, prefix_table, prefix, dim ** -0.5, t)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind,batch,longest,prefix", [
+    ((8, 0, 64, 1, 16), 2, 120, 0), ((8, 0, 128, 1, 16), 1, 9000, 0), ((4, 32, 128, 4, 16), 8, 6000, 0),
+    ((8, 0, 128, 4, 16), 40, 20, 12000), ((8, 0, 64, 4, 16), 20, 20, 16000)])
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("period", [32, 200, 1 << 20])
+def test_attention_values_that_fall_as_logits_rise(kind, batch, longest, prefix, period, back, t):
+    """Over each `period` keys (or all) logits rise by 60, which is a factor of
+    2^86 in p, and values fall by 2^40, or the other way round."""
+    bits, group, dim, heads, page = kind
+    per, shared = -(-longest // page), -(-prefix // page)
+    cache = filled(kind, batch * per + shared, 3)
+    pages = torch.arange(cache.pages, dtype=torch.int32, device="cuda")
+    prefix_table, table = pages[:shared].contiguous(), pages[shared:].view(batch, per)
+    q = torch.randn(batch, 1, heads * 4, dim, generator=generator(9), device="cuda").to(TYPES[t])
+    q[..., 0] = 16
+    top = 127 if bits == 8 else 7
+    cache.k.fill_(0 if bits == 8 else 0x88)
+    cache.k[..., 0] = top if bits == 8 else 0x8F
+    n = (shared if prefix else per) * page
+    at = (torch.arange(n, device="cuda") % period / min(n, period)).view(-1, 1, page, 1)
+    rise = 1 - at if back else at
+    for row in [prefix_table] if prefix else list(table):
+        cache.k_scale[row.long()] = (60 * dim ** 0.5 / (16 * top) * rise).expand(-1, heads, -1, cache.k_scale.shape[-1])
+        cache.v_scale[row.long()] *= 2.0 ** (-40 * rise)
+    if prefix:  # what follows the prefix has logits of 0 and weighs nothing
+        cache.k_scale[shared:] = 0
+        cache.v_scale[shared:] *= 2.0 ** -40
+    lens = torch.full((batch,), longest, dtype=torch.int32, device="cuda")
+    got = ops.KVAttention(cache, heads * 4).exec(q, table, lens, prefix_table=prefix_table, prefix_len=prefix)
+    near_by_weight(got, cache, q, table, lens, prefix_table, prefix, dim ** -0.5, t)
