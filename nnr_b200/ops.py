@@ -513,7 +513,8 @@ class _Fixed:
     _fixed = frozenset()
 
     def __setattr__(self, name, value):
-        if name in self._fixed and name in self.__dict__:
+        # (x.k *= 2 sets k to itself)
+        if name in self._fixed and self.__dict__.get(name, value) is not value:
             raise AttributeError(f"{name} is fixed once the {type(self).__name__} is made")
         super().__setattr__(name, value)
 

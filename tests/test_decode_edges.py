@@ -4,6 +4,7 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
 
 from nnr_b200 import ops
 
@@ -45,3 +46,12 @@ def test_what_calls_rely_on_is_set_once(kind, names):
         with pytest.raises(AttributeError, match=name):
             setattr(x, name, 2)
         assert getattr(x, name) == 1
+
+
+def test_a_buffer_may_be_changed_in_place():
+    cache = ops.KVCache.__new__(ops.KVCache)
+    cache.k_scale = buffer = torch.ones(3)
+    cache.k_scale *= 2
+    assert cache.k_scale is buffer and (buffer == 2).all()
+    with pytest.raises(AttributeError):
+        cache.k_scale = cache.k_scale * 2
