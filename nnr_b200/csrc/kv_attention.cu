@@ -89,14 +89,14 @@ size_t lay_out(const nnrcu_kv_cache& c, const nnrcu_kv_attention_desc& d, Args* 
 
 // Joins the segments of each row: WARPS warps a row, which share its segments
 // out, four channels a lane. A lane
-// holds one segment's factor, so that the segments' sums are loaded without
-// waiting for one another. Starts while the attention ends, and then takes 3 to
+// holds one segment's share in the result, so that the segments' means are
+// loaded without waiting for one another. Starts while the attention ends, and then takes 3 to
 // 4 us, which is latency: lengths, factors, sums, one after the other. The order
 // of the sums depends on the segments alone.
 template <int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args p) {
   static_assert(WARPS == 1 || WARPS == 4, "a warp or the block");
-  __shared__ float tops[4], totals[4];
+  __shared__ float refs[4], totals[4];
   __shared__ float4 sums[WARPS > 1 ? 4 : 1][2][32];
   const int row = (int)(blockIdx.x * (4 / WARPS)) + (WARPS == 1 ? threadIdx.x >> 5 : 0);
   const int lane = threadIdx.x & 31, warp = WARPS == 1 ? 0 : threadIdx.x >> 5;
@@ -128,27 +128,37 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
   }
   attn::pdl_wait();  // in every thread: what follows on the stream relies on it
   if (!p.prefix_len && count[0] == 1) return;  // written already
-  float top = -INFINITY;
+  // The sum of p over the warp's segments, and what it is relative to.
+  float2 held[2];  // this lane's first segment of its own part and of the prefix
+  float ref = -INFINITY, total = 0.f;
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    for (int s = warp + lane * WARPS; s < count[k]; s += 32 * WARPS) top = fmaxf(top, ml[k][s * step[k]].x);
-  for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, w));
-  if constexpr (WARPS > 1) {
-    if (lane == 0) tops[warp] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  for (int k = 0; k < 2; ++k) {
+    const int s = warp + lane * WARPS;
+    held[k] = s < count[k] ? ml[k][s * step[k]] : make_float2(-INFINITY, 0.f);
   }
-  const float ref = top == -INFINITY ? 0.f : top;
-  float total = 0.f;
+  auto add = [&](const float2 x) {
+    const float next = fmaxf(ref, x.y == 0.f ? -INFINITY : x.x), base = next == -INFINITY ? 0.f : next;
+    total = total * attn::exp2_fast(ref - base) + (x.y == 0.f ? 0.f : x.y * attn::exp2_fast(x.x - base));
+    ref = next;
+  };
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    add(held[k]);
+    for (int s = warp + (lane + 32) * WARPS; s < count[k]; s += 32 * WARPS) add(ml[k][s * step[k]]);
+  }
+  const float mine = ref;
+  for (int w = 16; w; w >>= 1) ref = fmaxf(ref, __shfl_xor_sync(~0u, ref, w));
+  total *= attn::exp2_fast(mine - (ref == -INFINITY ? 0.f : ref));
+  for (int w = 16; w; w >>= 1) total += __shfl_xor_sync(~0u, total, w);
+  const float base = ref == -INFINITY ? 0.f : ref, part = total == 0.f ? 0.f : 1.f / total;
   float4 sum[2] = {};
 #pragma unroll
   for (int k = 0; k < 2; ++k)
     for (int s0 = warp; s0 < count[k]; s0 += 32 * WARPS) {  // segments s0, s0 + WARPS, ...
       float f = 0.f;
       if (s0 + lane * WARPS < count[k]) {
-        const float2 x = ml[k][(s0 + lane * WARPS) * step[k]];
-        if (x.y != 0.f) f = attn::exp2_fast(x.x - ref);
-        total += f * x.y;
+        const float2 x = s0 == warp ? held[k] : ml[k][(s0 + lane * WARPS) * step[k]];
+        if (x.y != 0.f) f = x.y * attn::exp2_fast(x.x - base) * part;
       }
       const int n = min(32, (count[k] - s0 + WARPS - 1) / WARPS);
       const float* from = o[k] + (long long)s0 * step[k] * p.dim + lane * 4;
@@ -164,29 +174,36 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
           }
       }
     }
-  for (int w = 16; w; w >>= 1) total += __shfl_xor_sync(~0u, total, w);
-  if constexpr (WARPS > 1) {
-    if (lane == 0) totals[warp] = total;
+  if constexpr (WARPS > 1) {  // the warps' means, as the segments'
+    if (lane == 0) refs[warp] = ref, totals[warp] = total;
     sums[warp][0][lane] = sum[0], sums[warp][1][lane] = sum[1];
     __syncthreads();
     if (warp) return;
-    total = totals[0];
-    for (int w = 1; w < 4; ++w) {
-      total += totals[w];
+    const float top = fmaxf(fmaxf(refs[0], refs[1]), fmaxf(refs[2], refs[3]));
+    float f[4], all = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      f[w] = totals[w] == 0.f ? 0.f : totals[w] * attn::exp2_fast(refs[w] - (top == -INFINITY ? 0.f : top));
+      all += f[w];
+    }
+    const float of_all = all == 0.f ? 0.f : 1.f / all;
+    sum[0] = sum[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float g = f[w] * of_all;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float4 x = sums[w][e][lane];
-        sum[e].x += x.x, sum[e].y += x.y, sum[e].z += x.z, sum[e].w += x.w;
+        sum[e].x += x.x * g, sum[e].y += x.y * g, sum[e].z += x.z * g, sum[e].w += x.w * g;
       }
     }
   }
-  const float part = total == 0.f ? 0.f : 1.f / total;
 #pragma unroll
   for (int e = 0; e < 2; ++e)
     if (e * 128 + lane * 4 < p.dim) {
       const long long at = (long long)row * p.dim + e * 128 + lane * 4;
-      attn::store_y(p, at, sum[e].x * part), attn::store_y(p, at + 1, sum[e].y * part);
-      attn::store_y(p, at + 2, sum[e].z * part), attn::store_y(p, at + 3, sum[e].w * part);
+      attn::store_y(p, at, sum[e].x), attn::store_y(p, at + 1, sum[e].y);
+      attn::store_y(p, at + 2, sum[e].z), attn::store_y(p, at + 3, sum[e].w);
     }
 }
 

@@ -64,8 +64,8 @@ struct Args {
   // 128 keys. All units' quads in a row are shared out evenly over `grid`
   // blocks; one block's stretch of one unit is a segment, numbered unit +
   // block, which no other segment has. Each leaves for its rows
-  //   ml: the largest logit (log2 units) and the sum of weights,
-  //   o:  the sum of weights times values,
+  //   ml: what p is relative to (a logit, log2 units) and the sum of p,
+  //   o:  the mean of the values by p (their sum might pass fp32's range),
   // unless it is all of its unit and there is nothing to join.
   struct Part {
     int rows, blocks, units, grid;  // rows of a block; blocks of one head; units of one sequence
@@ -352,6 +352,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
   __shared__ long long row_q[C::kRows], row_y[C::kRows];
   __shared__ int row_lo[C::kRows], row_hi[C::kRows];
   __shared__ float2 warp_ml[kWarps][C::kRows];
+  __shared__ float4 row_part[C::kRows];
   for (;;) {
     const int n_quads = min(at.quads - at.quad, stop - at_quad);
     const int head = at.unit / w.blocks, first_row = (at.unit - head * w.blocks) * C::kRows;
@@ -779,39 +780,47 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
         x += __shfl_xor_sync(~0u, x, 8);
         x += __shfl_xor_sync(~0u, x, 16);
         const int r = 8 * n + 2 * t + e;
-        const float real = __uint_as_float((254 - unit[n][e]) << 23);
+        const float real = __uint_as_float((254 - unit[n][e]) << 23), part = x == 0.f ? 0.f : 1.f / x;
         if (g == 0) warp_ml[warp][r] = make_float2(ref[n][e], x);
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) {
           const int at = BITS == 8 ? i * 16 + 2 * g : i / 2 * 32 + 4 * g + 2 * (i % 2);
-          *reinterpret_cast<float2*>(mo + r * C::kMergeRow + at) = make_float2(o[i][n][e] * real, o[i][n][2 + e] * real);
+          *reinterpret_cast<float2*>(mo + r * C::kMergeRow + at) =
+              make_float2(o[i][n][e] * part * real, o[i][n][2 + e] * part * real);
         }
       }
     __syncthreads();
     const bool whole = n_quads == at.quads && !p.prefix_len;
     const long long segment = ((own ? (long long)at.b * w.units : 0) + at.unit + blockIdx.x) * C::kRows;
-    for (int x = threadIdx.x; x < C::kRows * DP; x += kWarps * 32) {
-      const int r = x / DP, c = x % DP;
-      const long long row = row_y[r];
-      if (row < 0 || c >= dim) continue;
-      float most = -INFINITY, sum = 0.f, total = 0.f;
+    if (threadIdx.x < C::kRows) {  // the warps' shares in a row
+      const int r = threadIdx.x;
+      float most = -INFINITY, total = 0.f, f[kWarps];
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) most = fmaxf(most, warp_ml[i][r].x);
       const float base = most == -INFINITY ? 0.f : most;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) {
-        const float f = exp2_fast(warp_ml[i][r].x - base);
-        if (warp_ml[i][r].y != 0.f) {
-          total += warp_ml[i][r].y * f;
-          sum += reinterpret_cast<const float*>(smem)[(i * C::kRows + r) * C::kMergeRow + c] * f;
-        }
+        f[i] = warp_ml[i][r].y == 0.f ? 0.f : warp_ml[i][r].y * exp2_fast(warp_ml[i][r].x - base);
+        total += f[i];
       }
-      if (whole) {
-        store_y(p, row * dim + c, total == 0.f ? 0.f : sum / total);
-      } else {
-        if (c == 0) w.ml[segment + r] = make_float2(most, total);
-        w.o[(segment + r) * dim + c] = sum;
-      }
+      const float part = total == 0.f ? 0.f : 1.f / total;
+      row_part[r] = make_float4(f[0] * part, f[1] * part, f[2] * part, f[3] * part);
+      if (!whole && row_y[r] >= 0) w.ml[segment + r] = make_float2(most, total);
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < C::kRows * DP; x += kWarps * 32) {
+      const int r = x / DP, c = x % DP;
+      const long long row = row_y[r];
+      if (row < 0 || c >= dim) continue;
+      static_assert(kWarps == 4, "a share each");
+      const float* const mean = reinterpret_cast<const float*>(smem) + r * C::kMergeRow + c;
+      constexpr int kFar = C::kRows * C::kMergeRow;
+      const float4 f = row_part[r];
+      const float y = (mean[0] * f.x + mean[kFar] * f.y) + (mean[2 * kFar] * f.z + mean[3 * kFar] * f.w);
+      if (whole)
+        store_y(p, row * dim + c, y);
+      else
+        w.o[(segment + r) * dim + c] = y;
     }
     at_quad += n_quads;
     if (at_quad >= stop || !next_unit(p, own, w.units, at)) break;

@@ -384,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
       const bool whole = n_quads == at.quads && !p.prefix_len;
       const long long segment = ((own ? (long long)at.b * w.units : 0) + at.unit + blockIdx.x) * kM + r;
       const float real = tiles > 0 && ok && sum != 0.f ? __uint_as_float((254 - unit) << 23) : 0.f;
-      const float f = whole && real != 0.f ? real / sum : real;
+      const float part = real == 0.f ? 0.f : 1.f / sum;  // the mean is kept, as in kv_attention.cuh
       // O by 32 channels through shared memory (every product has ended), so
       // that a store is one row's 32 and not one channel of 32 rows.
       float* const turn = reinterpret_cast<float*>(smem + L::kK) + warp * 32 * 33;
@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
           for (int j = 0; j < 32; ++j) o[j] = 0;
         }
 #pragma unroll
-        for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = __uint_as_float(o[j]) * f;
+        for (int j = 0; j < 32; ++j) turn[lane * 33 + j] = __uint_as_float(o[j]) * part * real;
         __syncwarp();
         if (whole) {
 #pragma unroll 4

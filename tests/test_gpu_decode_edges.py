@@ -217,3 +217,23 @@ def test_attention_values_that_fall_as_logits_rise(kind, batch, longest, prefix,
     lens = torch.full((batch,), longest, dtype=torch.int32, device="cuda")
     got = ops.KVAttention(cache, heads * 4).exec(q, table, lens, prefix_table=prefix_table, prefix_len=prefix)
     near_by_weight(got, cache, q, table, lens, prefix_table, prefix, dim ** -0.5, t)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("kind,batch,longest,prefix", [
+    ((8, 0, 64, 1, 16), 2, 120, 0), ((4, 32, 128, 1, 16), 2, 900, 0), ((8, 0, 256, 1, 16), 2, 900, 0),
+    ((8, 0, 128, 8, 16), 1, 9000, 0), ((8, 0, 128, 4, 16), 40, 20, 6000), ((8, 0, 64, 4, 16), 3, 20, 6000)])
+def test_attention_of_values_near_the_largest(kind, batch, longest, prefix, t):
+    """A mean of values is no larger than they are, however large their sum."""
+    bits, group, dim, heads, page = kind
+    per, shared = -(-longest // page), -(-prefix // page)
+    cache = filled(kind, batch * per + shared, 3)
+    pages = torch.arange(cache.pages, dtype=torch.int32, device="cuda")
+    prefix_table, table = pages[:shared].contiguous(), pages[shared:].view(batch, per)
+    cache.v_scale.fill_(2.6e36 if bits == 8 else 4.7e37)  # values up to 3.3e38
+    cache.v.clamp_(min=1) if bits == 8 else cache.v.bitwise_or_(0x99)
+    cache.k_scale *= 0.1  # many keys of about the same weight
+    lens = torch.full((batch,), longest, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, 1, heads * 4, dim, generator=generator(9), device="cuda").to(TYPES[t])
+    got = ops.KVAttention(cache, heads * 4).exec(q, table, lens, prefix_table=prefix_table, prefix_len=prefix)
+    near_by_weight(got, cache, q, table, lens, prefix_table, prefix, dim ** -0.5, t)
