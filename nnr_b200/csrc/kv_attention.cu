@@ -291,8 +291,7 @@ int nnrcu_kv_attention_run(const nnrcu_kv_cache* cache, const nnrcu_kv_attention
   p.max_len = d.max_len;
   p.prefix_len = d.prefix_len;
   p.window = d.window;
-  // a scale of 0 keeps every logit at 0, and hidden ones hidden
-  p.scale_log2 = std::max(std::fabs(d.scale) * 1.44269504088896340736f, 0x1p-126f);
+  p.scale_log2 = std::fabs(d.scale) * 1.44269504088896340736f;
   p.q_sign = d.scale < 0 ? -1.f : 1.f;
   p.run = cache->page_size % 32 == 0 ? 32 : (cache->page_size % 16 == 0 ? 16 : 1);
   p.dtype = d.dtype;

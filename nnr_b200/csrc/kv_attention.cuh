@@ -55,7 +55,7 @@ struct Args {
   const int32_t* lens;
   const int32_t* prefix_table;
   int max_len, prefix_len, window;
-  float scale_log2;       // |scale| * log2(e), not 0
+  float scale_log2;       // |scale| * log2(e)
   float q_sign;           // of scale
   int q_wide;             // q may be read 4 or 8 channels at a time, as a lane wants them
   int q_wide16;           // and 8 16-bit channels
@@ -464,7 +464,10 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
     // come, each row scaled by a power of two to lie below 2^15
     uint32_t qf[C::kQShared ? 1 : PARTS][NT][C::kQShared ? 1 : DP / 16][2];
     uint2* const q_shared = reinterpret_cast<uint2*>(smem + C::kBody);
-    float row_scale[NT][2];  // of rows 2 t + e: what turns a logit's product into log2 units
+    // Of rows 2 t + e: what their logits are in. A power of two, so that the
+    // largest logit and what it is less than by one multiplication and addition
+    // are the same number however large it is; key scales carry the rest.
+    float row_scale[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const bool real = row_y[8 * n + g] >= 0;
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
       most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
       const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 15u), 254u);
       const float f = __uint_as_float((268 - exponent) << 23) * p.q_sign;  // 2^(14 - E), E = exponent - 127
-      const float back = fmaxf(__uint_as_float((exponent - 14) << 23) * p.scale_log2, 0x1p-126f);
+      const float back = __uint_as_float((exponent - 14) << 23);
 #pragma unroll
       for (int e = 0; e < 2; ++e) row_scale[n][e] = __shfl_sync(~0u, back, (2 * t + e) * 4);
 #pragma unroll
@@ -588,7 +591,8 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
               if constexpr (GROUPED) {  // 8 bits: two chunks are a group; 4 bits: one is
                 const int grp = BITS == 4 ? c + cc : c / 2;
                 if ((BITS == 4 || cc == 1) && grp < groups) {
-                  const float f0 = ks[(i * 16 + g) * C::kGroups + grp], f1 = ks[(i * 16 + 8 + g) * C::kGroups + grp];
+                  const float f0 = ks[(i * 16 + g) * C::kGroups + grp] * p.scale_log2;
+                  const float f1 = ks[(i * 16 + 8 + g) * C::kGroups + grp] * p.scale_log2;
 #pragma unroll
                   for (int n = 0; n < NT; ++n) {
                     s[i][n][0] = fmaf(part[n][0], f0, s[i][n][0]), s[i][n][1] = fmaf(part[n][1], f0, s[i][n][1]);
@@ -600,7 +604,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
           }
         }
         if constexpr (!GROUPED) {
-          const float f0 = ks[i * 16 + g], f1 = ks[i * 16 + 8 + g];
+          const float f0 = ks[i * 16 + g] * p.scale_log2, f1 = ks[i * 16 + 8 + g] * p.scale_log2;
 #pragma unroll
           for (int n = 0; n < NT; ++n) s[i][n][0] *= f0, s[i][n][1] *= f0, s[i][n][2] *= f1, s[i][n][3] *= f1;
         }

@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
         most = fmaxf(most, other(most, ok));
         const uint32_t exponent = min(max(__float_as_uint(most) >> 23, 15u), 254u);
         const float f = __uint_as_float((268 - exponent) << 23) * p.q_sign;
-        row_scale = fmaxf(__uint_as_float((exponent - 14) << 23) * p.scale_log2, 0x1p-126f);
+        row_scale = __uint_as_float((exponent - 14) << 23);  // key scales carry the rest, see kv_attention.cuh
 #pragma unroll
         for (int c = 0; c < DIM / 16; ++c) {
           uint32_t y[4];
@@ -496,6 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
         const int g = done + n, slot = g % kRing;
         if (!__all_sync(~0u, g == 0 || wait(K_EMPTY, g - 1))) return false;
         const int j = begin + n * kN + key;
+        scales[slot * kN + key] *= p.scale_log2;
         const uint32_t r_bits = __float_as_uint(scales[(kRing + slot) * kN + key]) & 0x7FFFFFFFu;
         const bool counts = j >= any_lo && j < any_hi && r_bits < 0x7F800000u;  // a hidden key's is 0
         const uint32_t widest = __reduce_max_sync(~0u, counts ? r_bits >> 23 : 0u);

@@ -237,3 +237,23 @@ def test_attention_of_values_near_the_largest(kind, batch, longest, prefix, t):
     q = torch.randn(batch, 1, heads * 4, dim, generator=generator(9), device="cuda").to(TYPES[t])
     got = ops.KVAttention(cache, heads * 4).exec(q, table, lens, prefix_table=prefix_table, prefix_len=prefix)
     near_by_weight(got, cache, q, table, lens, prefix_table, prefix, dim ** -0.5, t)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind,batch,prefix", [((8, 0, 64, 1, 16), 2, 0), ((8, 0, 64, 1, 16), 40, 500),
+                                               ((4, 32, 128, 1, 16), 2, 0), ((8, 0, 256, 1, 16), 2, 0)])
+@pytest.mark.parametrize("size", [1e3, 1e4, 3e4])
+@pytest.mark.parametrize("scale", [None, -0.3, 1.7, 0.0])
+def test_attention_logits_far_past_fp32_steps_of_one(kind, batch, prefix, size, scale, t):
+    """Queries and keys of 1e4 have logits of 1e8, where fp32 has steps of 8 and
+    more: the largest alone is left, and its value comes out."""
+    cache = filled(kind, batch * 8 + 34, 3)
+    cache.k_scale.mul_(size)
+    table, prefix_table = layout(cache, batch, 120, prefix, 3)
+    lens = torch.full((batch,), 120, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, 1, 4, kind[2], generator=generator(9), device="cuda").clamp(-2, 2)
+    q = (q * size).to(TYPES[t])
+    got = ops.KVAttention(cache, 4, scale=scale).exec(q, table, lens, prefix_table=prefix_table, prefix_len=prefix)
+    scale = kind[2] ** -0.5 if scale is None else scale
+    want, slack = attention_ref(cache, q, table, lens, prefix_table, prefix, 0, scale, t)
+    near(got, want, slack, t)
