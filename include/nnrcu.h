@@ -398,8 +398,9 @@ int nnrcu_kv_cache_read(const nnrcu_kv_cache* cache, const int64_t* slots, long 
  *   y  the same, contiguous
  * lens on the device are at most max_len (larger ones are cut to it, negative
  * ones to 0, and reported as device status 17); a page number outside the
- * cache hides its tokens (device status 18). Device status 19: a wait inside a
- * kernel ran out of time. */
+ * cache hides its tokens (device status 18, unless no query sees them: entries
+ * for pages that every window has left behind, or past a sequence's end, may
+ * hold anything). Device status 19: a wait inside a kernel ran out of time. */
 typedef struct nnrcu_kv_attention_desc {
   int batch, q_len, q_heads, dtype;
   long long q_batch_stride, q_token_stride, q_head_stride;

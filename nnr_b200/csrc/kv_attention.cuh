@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
         const int page = next_page;
         next_page = page_of(n + 1);
         const bool in = j < end, there = in && (unsigned)page < (unsigned)p.pages;
-        if (in && !there) report(p.status, ST_PAGE);
+        if (in && !there && j >= any_lo) report(p.status, ST_PAGE);  // a key that no row sees may lack its page
         next_valid = __ballot_sync(~0u, there);
         row = there ? ((long long)page * p.heads + head) * p.page.d + (j - div_by(j, p.page) * p.page.d) : 0;
         copy(slot, p.k, p.k_scale);

@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
           const int j = begin + n * kN + key, page = next_page, slot = (done + n) % kRing;
           next_page = page_of(n + 1);
           const bool there = j < end && (unsigned)page < (unsigned)p.pages;
-          if (j < end && !there) report(p.status, ST_PAGE);
+          if (j < end && !there && j >= any_lo) report(p.status, ST_PAGE);  // as in kv_attention.cuh
           const uint32_t mask = __ballot_sync(~0u, there);
           rows_k = there ? ((long long)page * p.heads + head) * p.page.d + (j - div_by(j, p.page) * p.page.d) : 0;
           copy_async<4>(ptx::smem_u32(scales + slot * kN + key), p.k_scale + rows_k, there);

@@ -257,3 +257,31 @@ def test_attention_logits_far_past_fp32_steps_of_one(kind, batch, prefix, size, 
     scale = kind[2] ** -0.5 if scale is None else scale
     want, slack = attention_ref(cache, q, table, lens, prefix_table, prefix, 0, scale, t)
     near(got, want, slack, t)
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("kind,batch,q_len,prefix,window", [((8, 0, 128, 2, 16), 2, 2, 0, 60), ((8, 0, 64, 2, 5), 3, 1, 0, 40),
+                                                           ((4, 32, 128, 2, 16), 2, 3, 0, 1), ((8, 0, 128, 2, 16), 40, 1, 203, 150),
+                                                           ((8, 0, 64, 1, 16), 2, 48, 0, 7)])
+def test_attention_pages_that_no_window_reaches_may_be_gone(kind, batch, q_len, prefix, window, t):
+    """A table may hold -1 for a page that every window has left behind, and
+    beyond a sequence's end; that is no error."""
+    page = kind[4]
+    per, shared = -(-100 // page), -(-prefix // page)
+    cache = filled(kind, batch * per + shared + 3, 5)
+    table, prefix_table = layout(cache, batch, 100, prefix, 4)
+    table = table.contiguous()
+    lens = torch.randint(70, 101, (batch,), generator=generator(6), device="cuda", dtype=torch.int32)
+    q = torch.randn(batch, q_len, 8, kind[2], generator=generator(4), device="cuda").to(TYPES[t])
+    op = ops.KVAttention(cache, 8, window=window)
+    kw = dict(max_len=100, prefix_len=prefix)
+    want = op.exec(q, table, lens, prefix_table=prefix_table, **kw)
+    first = prefix + lens - q_len - window + 1  # the first position that a sequence's first query sees
+    for b in range(batch):
+        table[b, :max(0, int(first[b]) - prefix) // page] = -1
+        table[b, -(-int(lens[b]) // page):] = -1
+    prefix_table[:min(prefix, max(0, int(first.min()))) // page] = -1
+    assert (table == -1).any()
+    assert torch.equal(op.exec(q, table, lens, prefix_table=prefix_table, **kw), want)
+    torch.cuda.synchronize()
+    assert ops.device_status() == 0
