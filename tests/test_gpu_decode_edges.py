@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from nnr_b200 import ops
-from test_gpu_decode import HALF, TYPES, attention_ref, filled, generator, layout, near, values
+from test_gpu_decode import HALF, TYPES, attention_ref, filled, generator, layout, near, values, weights
 
 pytestmark = pytest.mark.gpu
 
@@ -285,3 +285,50 @@ def test_attention_pages_that_no_window_reaches_may_be_gone(kind, batch, q_len, 
     assert torch.equal(op.exec(q, table, lens, prefix_table=prefix_table, **kw), want)
     torch.cuda.synchronize()
     assert ops.device_status() == 0
+
+
+@pytest.mark.parametrize("kind,batch,prefix", [((8, 0, 128, 2, 16), 3, 0), ((4, 0, 64, 2, 16), 40, 300)])
+def test_a_step_in_a_cuda_graph_and_on_two_streams(kind, batch, prefix):
+    """A projection, the cache's write and attention, captured and replayed with
+    other inputs and lengths; and two such steps at once."""
+    bits, group, dim, heads, page = kind
+    hidden, q_heads = 96, heads * 4
+    cache = filled(kind, batch * 4 + 30, 3)
+    table, prefix_table = layout(cache, batch, 60, prefix, 1)
+    b, s, z, c = weights((q_heads + 2 * heads) * dim, hidden, 32, "bf16", True, True, 1)
+    linear, attention = ops.MatMulNBits(b, s * 0.1, hidden, zero_points=z, bias=c), ops.KVAttention(cache, q_heads)
+    x = torch.randn(batch, hidden, generator=generator(2), device="cuda").bfloat16()
+    lens = torch.full((batch,), 7, dtype=torch.int32, device="cuda")
+
+    def slots():
+        at = lens.long() - 1
+        return table.gather(1, (at // page)[:, None])[:, 0].long() * page + at % page
+
+    def step(x, stream=None):
+        qkv = linear.exec(x, stream=stream).view(batch, -1, dim)
+        cache.write(qkv[:, q_heads:q_heads + heads], qkv[:, q_heads + heads:], to, stream=stream)
+        return attention.exec(qkv[:, None, :q_heads], table, lens, max_len=60, prefix_table=prefix_table,
+                              prefix_len=prefix, stream=stream)
+
+    to = slots()
+    step(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step(x)
+    for held in (7, 20, 60):
+        lens.fill_(held)
+        to.copy_(slots())
+        x.normal_(generator=generator(held))
+        graph.replay()
+        assert torch.equal(y, step(x))
+    want, other = step(x), torch.randn(batch, hidden, generator=generator(3), device="cuda").bfloat16()
+    q = [linear.exec(a).view(batch, -1, dim)[:, None, :q_heads] for a in (x, other)]
+    kw = dict(max_len=60, prefix_table=prefix_table, prefix_len=prefix)
+    wants = [attention.exec(a, table, lens, **kw) for a in q]
+    streams = [torch.cuda.Stream() for _ in q]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = [attention.exec(a, table, lens, stream=st, **kw) for a, st in zip(q, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, wants))
+    assert torch.equal(wants[0], want)
