@@ -302,8 +302,10 @@ int nnrcu_kv_attention_run(const nnrcu_kv_cache* cache, const nnrcu_kv_attention
   p.q_wide = reinterpret_cast<uintptr_t>(q) % align == 0 && d.q_batch_stride % wide == 0 &&
              d.q_token_stride % wide == 0 && d.q_head_stride % wide == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const auto few = d.dtype == NNRCU_DT_F32 ? (cache->bits == 8 ? attn::launch_p2_b8 : attn::launch_p2_b4)
-                                           : (cache->bits == 8 ? attn::launch_p1_b8 : attn::launch_p1_b4);
+  const bool eight = cache->bits == 8;
+  const auto few = d.dtype == NNRCU_DT_F32   ? (eight ? attn::launch_f32_b8 : attn::launch_f32_b4)
+                   : d.dtype == NNRCU_DT_F16 ? (eight ? attn::launch_f16_b8 : attn::launch_f16_b4)
+                                             : (eight ? attn::launch_bf16_b8 : attn::launch_bf16_b4);
   auto launch = [&](const Args& a, bool own, cudaStream_t s) {
     return (own ? a.own : a.prefix).rows == 128 ? attn::launch_many(a, cache->bits, own, s) : few(a, own, s);
   };

@@ -89,7 +89,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // steps of 2^-39 below. So are the weights p_j r_j, by a unit of each row's that
 // puts the largest so far at 2^6 or more: a weight keeps 11 bits down to 2^-20
 // of the largest weight, whatever larger values the row all but leaves out.
-// PARTS = 2 (fp32 tensors) holds a value as the sum of two of them (22 bits).
+// A value of PARTS = 2 is the sum of two of them (22 bits): the weights of fp16
+// and fp32 tensors, and fp32 queries. One would be enough for bf16 results,
+// which keep 8 bits, but in fp16 it would cost as much as the result's own
+// rounding does (error against 64 bits, 32 sequences of 5000: 2.9e-4 of the
+// output with one, 2.1e-4 with two).
 template <int PARTS>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t (&out)[PARTS]) {
 #pragma unroll
@@ -158,8 +162,9 @@ constexpr int blocks_of_sm(int dim, bool fp32, int rows) {
   return fp32 && dim > 64 ? 2 : 3;
 }
 
-// Sizes of one kernel: head_dim padded to DP (EXACT: it is DP), 8 NT query rows.
-template <int PARTS, int BITS, bool GROUPED, int DP, bool EXACT, int NT>
+// Sizes of one kernel: fp16 parts of queries and of weights, head_dim padded to
+// DP (EXACT: it is DP), 8 NT query rows.
+template <int PARTS, int WPARTS, int BITS, bool GROUPED, int DP, bool EXACT, int NT>
 struct Cfg {
   static constexpr int kRows = 8 * NT;
   static constexpr int kRowBytes = DP * BITS / 8;
@@ -331,10 +336,10 @@ __device__ __forceinline__ void store_y(const Args& p, long long at, float v) {
 // (7 sequences, 20001 of 30000 visible, scales of 32 channels): 66 us, bound by
 // the warps' instructions (some 1340 a tile) and latencies, with 8 warps on an
 // SM, for which the registers suffice.
-template <int PARTS, int BITS, bool GROUPED, int DP, bool EXACT, int NT>
-__global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXACT, NT>::kBlocks)
+template <int PARTS, int WPARTS, int BITS, bool GROUPED, int DP, bool EXACT, int NT>
+__global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, WPARTS, BITS, GROUPED, DP, EXACT, NT>::kBlocks)
     attend_kernel(const __grid_constant__ Args p, const bool own) {
-  using C = Cfg<PARTS, BITS, GROUPED, DP, EXACT, NT>;
+  using C = Cfg<PARTS, WPARTS, BITS, GROUPED, DP, EXACT, NT>;
   constexpr int kOf = C::kChunkDim / 4;  // channels of a chunk that one lane holds
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -482,7 +487,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
         if (real && ch < dim && tiles > 0) {
           if (PARTS == 2)
             load_q<float, kOf>(x[c], p.q, at + ch, p.q_wide);
-          else if (p.dtype == NNRCU_DT_BF16)
+          else if (WPARTS == 1)
             load_q<__nv_bfloat16, kOf>(x[c], p.q, at + ch, p.q_wide);
           else
             load_q<__half, kOf>(x[c], p.q, at + ch, p.q_wide);
@@ -723,7 +728,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
       // o += D^T (p r)^T
 #pragma unroll
       for (int i = 0; i < kKeys / 16; ++i) {
-        uint32_t b[NT][PARTS][2];
+        uint32_t b[NT][WPARTS][2];
         auto weights = [&](int grp) {
           const float f0 = vs[(i * 16 + g) * C::kGroups + grp], f1 = vs[(i * 16 + 8 + g) * C::kGroups + grp];
 #pragma unroll
@@ -734,11 +739,11 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
               for (int e = 0; e < 4; ++e)
                 if (s[i][n][e] == 0.f) w[e] = 0.f;
             }
-            uint32_t x[PARTS], y[PARTS];
-            split_pair<PARTS>(w[0], w[1], x);
-            split_pair<PARTS>(w[2], w[3], y);
+            uint32_t x[WPARTS], y[WPARTS];
+            split_pair<WPARTS>(w[0], w[1], x);
+            split_pair<WPARTS>(w[2], w[3], y);
 #pragma unroll
-            for (int j = 0; j < PARTS; ++j) b[n][j][0] = transpose8x8(x[j]), b[n][j][1] = transpose8x8(y[j]);
+            for (int j = 0; j < WPARTS; ++j) b[n][j][0] = transpose8x8(x[j]), b[n][j][1] = transpose8x8(y[j]);
           }
         };
         if constexpr (!GROUPED) weights(0);
@@ -762,7 +767,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, BITS, GROUPED, DP, EXA
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                  for (int j = 0; j < PARTS; ++j) mma(o[(c + cc) * C::kSteps + st][n], a, b[n][j][0], b[n][j][1]);
+                  for (int j = 0; j < WPARTS; ++j) mma(o[(c + cc) * C::kSteps + st][n], a, b[n][j][0], b[n][j][1]);
               }
             }
           }
@@ -848,10 +853,10 @@ int launch_part(K kernel, const Args& p, bool own, int threads, int smem, cudaSt
   return cuda_check(cudaLaunchKernelEx(&cfg, kernel, p, own), "attention launch");
 }
 
-template <int PARTS, int BITS, bool GROUPED, int DP, bool EXACT, int NT>
+template <int PARTS, int WPARTS, int BITS, bool GROUPED, int DP, bool EXACT, int NT>
 int launch(const Args& p, bool own, cudaStream_t st) {
-  using C = Cfg<PARTS, BITS, GROUPED, DP, EXACT, NT>;
-  auto* kernel = attend_kernel<PARTS, BITS, GROUPED, DP, EXACT, NT>;
+  using C = Cfg<PARTS, WPARTS, BITS, GROUPED, DP, EXACT, NT>;
+  auto* kernel = attend_kernel<PARTS, WPARTS, BITS, GROUPED, DP, EXACT, NT>;
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may use its shared memory
   int device = 0;
   NNRCU_CUDA(cudaGetDevice(&device));
@@ -875,17 +880,17 @@ inline int rows_of_block(long long rows, int dim) {
 // The kernel for blocks of 128 rows (kv_attention_many.cu).
 int launch_many(const Args& p, int bits, bool own, cudaStream_t st);
 
-template <int PARTS, int BITS>
+template <int PARTS, int WPARTS, int BITS>
 int launch_for(const Args& p, bool own, cudaStream_t st) {
   const int rows = own ? p.own.rows : p.prefix.rows;
   auto go = [&](auto grouped, auto tiles) {
     constexpr bool G = decltype(grouped)::value;
     constexpr int N = decltype(tiles)::value;
-    if (p.dim == 64) return launch<PARTS, BITS, G, 64, true, N>(p, own, st);
-    if (p.dim == 128) return launch<PARTS, BITS, G, 128, true, N>(p, own, st);
-    if (p.dim < 64) return launch<PARTS, BITS, G, 64, false, N>(p, own, st);
-    if (p.dim < 128) return launch<PARTS, BITS, G, 128, false, N>(p, own, st);
-    return launch<PARTS, BITS, G, 256, false, 1>(p, own, st);  // rows_of_block gives no more
+    if (p.dim == 64) return launch<PARTS, WPARTS, BITS, G, 64, true, N>(p, own, st);
+    if (p.dim == 128) return launch<PARTS, WPARTS, BITS, G, 128, true, N>(p, own, st);
+    if (p.dim < 64) return launch<PARTS, WPARTS, BITS, G, 64, false, N>(p, own, st);
+    if (p.dim < 128) return launch<PARTS, WPARTS, BITS, G, 128, false, N>(p, own, st);
+    return launch<PARTS, WPARTS, BITS, G, 256, false, 1>(p, own, st);  // rows_of_block gives no more
   };
   auto by_rows = [&](auto grouped) {
     if (rows == 8) return go(grouped, std::integral_constant<int, 1>());
@@ -896,10 +901,12 @@ int launch_for(const Args& p, bool own, cudaStream_t st) {
 }
 
 // The instances of launch_for, each in a file of its own.
-int launch_p1_b8(const Args& p, bool own, cudaStream_t st);
-int launch_p1_b4(const Args& p, bool own, cudaStream_t st);
-int launch_p2_b8(const Args& p, bool own, cudaStream_t st);
-int launch_p2_b4(const Args& p, bool own, cudaStream_t st);
+int launch_bf16_b8(const Args& p, bool own, cudaStream_t st);
+int launch_bf16_b4(const Args& p, bool own, cudaStream_t st);
+int launch_f16_b8(const Args& p, bool own, cudaStream_t st);
+int launch_f16_b4(const Args& p, bool own, cudaStream_t st);
+int launch_f32_b8(const Args& p, bool own, cudaStream_t st);
+int launch_f32_b4(const Args& p, bool own, cudaStream_t st);
 
 }  // namespace attn
 }  // namespace nnrcu

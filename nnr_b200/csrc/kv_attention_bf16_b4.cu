@@ -1,0 +1,8 @@
+// The attention kernels for bf16 tensors over 4-bit codes (their instances compile apart).
+#include "kv_attention.cuh"
+
+namespace nnrcu {
+namespace attn {
+int launch_bf16_b4(const Args& p, bool own, cudaStream_t st) { return launch_for<1, 1, 4>(p, own, st); }
+}  // namespace attn
+}  // namespace nnrcu

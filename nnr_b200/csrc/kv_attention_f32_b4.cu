@@ -3,6 +3,6 @@
 
 namespace nnrcu {
 namespace attn {
-int launch_p2_b4(const Args& p, bool own, cudaStream_t st) { return launch_for<2, 4>(p, own, st); }
+int launch_f32_b4(const Args& p, bool own, cudaStream_t st) { return launch_for<2, 2, 4>(p, own, st); }
 }  // namespace attn
 }  // namespace nnrcu

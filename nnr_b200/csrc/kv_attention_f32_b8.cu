@@ -3,6 +3,6 @@
 
 namespace nnrcu {
 namespace attn {
-int launch_p2_b8(const Args& p, bool own, cudaStream_t st) { return launch_for<2, 8>(p, own, st); }
+int launch_f32_b8(const Args& p, bool own, cudaStream_t st) { return launch_for<2, 2, 8>(p, own, st); }
 }  // namespace attn
 }  // namespace nnrcu

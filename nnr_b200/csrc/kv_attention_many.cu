@@ -63,6 +63,26 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
+// As above, 16 columns, without waiting.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// D += A B with A in tensor memory: a lane a row, two 16-bit numbers a column.
+__device__ __forceinline__ void mma_f16_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, 1, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc)
+      : "memory");
+}
+
 // Waits for the phase with this parity without asking to be suspended (a tile
 // passes five such waits in turn); bounded as ptx::mbar_wait is.
 __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
@@ -100,7 +120,10 @@ __device__ __forceinline__ uint64_t desc_values(uint32_t addr) {
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
-template <int BITS, int DIM>
+// FINE: fp16 tensors, whose weights are held in two parts (see kv_attention.cuh).
+// The second goes to the 64 columns of tensor memory that S and O leave, as the
+// operand of a second product.
+template <int BITS, int DIM, bool FINE>
 __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_constant__ Args p, const bool own) {
   using L = Many<BITS, DIM>;
   constexpr int kChunks = DIM * BITS / 128;     // 16-byte chunks of a row's codes
@@ -130,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
   ptx::tc_fence_before();
   __syncthreads();
   ptx::tc_fence_after();
-  const uint32_t tmem = words[0], t_o = tmem + 256;
+  const uint32_t tmem = words[0], t_o = tmem + 256, t_rest = tmem + 384;
 
   const Args::Part w = own ? p.own : p.prefix;
   const Shares shares = shares_of(p, own, lane, 0);
@@ -199,10 +222,8 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
           if (row_y < 0) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[8 * c + j] = 0.f;
-          } else if (p.dtype == NNRCU_DT_BF16) {
-            load_q<__nv_bfloat16, 8>(x + 8 * c, p.q, at_q, p.q_wide16);
           } else {
-            load_q<__half, 8>(x + 8 * c, p.q, at_q, p.q_wide16);
+            load_q<std::conditional_t<FINE, __half, __nv_bfloat16>, 8>(x + 8 * c, p.q, at_q, p.q_wide16);
           }
         }
 #pragma unroll
@@ -333,6 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
             }
           }
         }
+        if constexpr (FINE) ptx::tc_fence_after();  // the last tile's second product has used what is written below
         const float base = ref == -INFINITY ? 0.f : ref, times = __uint_as_float(unit << 23);
         const float2 minus = make_float2(-base, -base), per_unit = make_float2(times, times);
 #pragma unroll
@@ -356,19 +378,23 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
               if (!((vis[c] >> (2 * j + 1)) & 1)) x[c][j].y = 0.f;
             }
           }
+          uint32_t rest[16];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {  // the chunk's 4 of the row's 16
             uint32_t y[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              uint32_t z[1];
-              split_pair<1>(x[c][4 * j + e].x, x[c][4 * j + e].y, z);
+              uint32_t z[FINE ? 2 : 1];
+              split_pair<FINE ? 2 : 1>(x[c][4 * j + e].x, x[c][4 * j + e].y, z);
               y[e] = z[0];
+              if constexpr (FINE) rest[4 * j + e] = z[1];
             }
             *reinterpret_cast<uint4*>(smem + L::kP + half * L::kSlab + chunk_at(r, 4 * c + j)) =
                 make_uint4(y[0], y[1], y[2], y[3]);
           }
+          if constexpr (FINE) tmem_st16(t_rest + lanes + 32 * half + 16 * c, rest);
         }
+        if constexpr (FINE) asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         ptx::fence_proxy_async_smem();
         ptx::tc_fence_before();
         ptx::mbar_arrive(bars + P_FULL);
@@ -561,6 +587,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
         for (int s = 0; s < kN / 16; ++s)
           ptx::mma_f16(t_o, ptx::umma_desc_sw128(base + L::kP + s / 4 * L::kSlab + s % 4 * 32),
                        desc_values(base + L::kV + s * 2048), idesc_o, n > 0 || s > 0);
+        if constexpr (FINE) {
+#pragma unroll
+          for (int s = 0; s < kN / 16; ++s)  // 16 keys are 8 columns
+            mma_f16_tmem(t_o, t_rest + 8 * s, desc_values(base + L::kV + s * 2048), idesc_o);
+        }
         ptx::mma_commit(bars + V_EMPTY);
         ptx::mma_commit(bars + O_DONE);
       }
@@ -580,9 +611,9 @@ __global__ void __launch_bounds__(kThreads, 1) attend_many_kernel(const __grid_c
   after_prefix(p, own);
 }
 
-template <int BITS, int DIM>
+template <int BITS, int DIM, bool FINE>
 int launch(const Args& p, bool own, cudaStream_t st) {
-  auto* kernel = attend_many_kernel<BITS, DIM>;
+  auto* kernel = attend_many_kernel<BITS, DIM, FINE>;
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel may use its shared memory
   int device = 0;
   NNRCU_CUDA(cudaGetDevice(&device));
@@ -596,8 +627,12 @@ int launch(const Args& p, bool own, cudaStream_t st) {
 }  // namespace
 
 int launch_many(const Args& p, int bits, bool own, cudaStream_t st) {
-  if (p.dim == 64) return bits == 8 ? launch<8, 64>(p, own, st) : launch<4, 64>(p, own, st);
-  return bits == 8 ? launch<8, 128>(p, own, st) : launch<4, 128>(p, own, st);
+  auto go = [&](auto fine) {
+    constexpr bool F = decltype(fine)::value;
+    if (p.dim == 64) return bits == 8 ? launch<8, 64, F>(p, own, st) : launch<4, 64, F>(p, own, st);
+    return bits == 8 ? launch<8, 128, F>(p, own, st) : launch<4, 128, F>(p, own, st);
+  };
+  return p.dtype == NNRCU_DT_F16 ? go(std::true_type()) : go(std::false_type());
 }
 
 }  // namespace attn

@@ -332,3 +332,23 @@ def test_a_step_in_a_cuda_graph_and_on_two_streams(kind, batch, prefix):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, wants))
     assert torch.equal(wants[0], want)
+
+
+@pytest.mark.parametrize("kind,batch,longest,prefix", [
+    ((8, 0, 128, 2, 16), 3, 1, 0), ((8, 0, 64, 1, 16), 5, 3, 0), ((4, 32, 128, 2, 16), 3, 300, 0), ((8, 32, 64, 2, 16), 2, 40, 0),
+    ((4, 0, 256, 1, 16), 2, 100, 0), ((8, 0, 128, 2, 16), 40, 2, 500), ((8, 0, 64, 2, 16), 40, 2, 130),
+    ((4, 0, 128, 4, 16), 40, 20, 9000), ((4, 0, 64, 4, 16), 70, 20, 9000)])
+def test_attention_in_fp16_is_off_by_its_rounding_only(kind, batch, longest, prefix):
+    """As test_gpu_decode's bound, but with weights of 22 bits, not of fp16's 11."""
+    bits, group, dim, heads, page = kind
+    per, shared = -(-longest // page), -(-prefix // page)
+    cache = filled(kind, batch * per + shared, 11)
+    table, prefix_table = layout(cache, batch, longest, prefix, 4)
+    lens = torch.full((batch,), longest, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, 1, heads * 4, dim, generator=generator(4), device="cuda").half()
+    got = ops.KVAttention(cache, heads * 4).exec(q, table, lens, prefix_table=prefix_table, prefix_len=prefix)
+    want, slack = attention_ref(cache, q, table, lens, prefix_table, prefix, 0, dim ** -0.5, "f32")
+    near(got, want, slack, "f16")  # fp32's slack has 2^-20 for exp and the weights
+    if longest == 1 and not prefix:
+        v = values(cache, "v")[table[:, 0].long(), 0].half()
+        assert torch.equal(got[:, 0], v.repeat_interleave(4, 1))
