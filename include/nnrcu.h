@@ -394,6 +394,9 @@ int nnrcu_kv_cache_read(const nnrcu_kv_cache* cache, const int64_t* slots, long 
  * one that sees nothing gives zeros. Query head h reads cache head
  * h / (q_heads / heads). The shared prefix is worked through once for the
  * whole batch, then joined with each sequence's own part.
+ * Logits, sums and results before rounding are fp32. As operands of the second
+ * product, softmax weights (times their values' scales) keep 22 bits, those of
+ * bf16 tensors 11, down to 2^-20 of the row's largest; fp32 queries keep 22.
  *   q  [batch][q_len][q_heads][head_dim], strides in elements, channels contiguous
  *   y  the same, contiguous
  * lens on the device are at most max_len (larger ones are cut to it, negative

@@ -37,10 +37,12 @@ int check(const nnrcu_kv_cache* c, const nnrcu_kv_attention_desc* d, bool buffer
 }
 
 // Rows of a key/value head from which the blocks of 128 are worth their fixed
-// cost. A prefix of 16384 keys, 8 heads, few against many (us): 8 bits and
-// dimension 128, 32 rows 41.2 and 40.1, 40 rows 48.9 and 40.3; 4 bits, 24 rows
-// 31.3 and 38.0, 48 rows 43.0 and 38.6; dimension 64, 24 rows 24.6 and 32.3,
-// 48 rows 32.1 and 32.6. 16 sequences of 8192 with 32 rows: 97 and 116.
+// cost. A prefix of 16384 keys, 8 heads, few against many (us), bf16: 8 bits and
+// dimension 128, 32 rows 40.8 and 41.1, 40 rows 50.5 and 41.4; 16 sequences of
+// 8192, 32 rows 59 and 68, 40 rows 74 and 68. With less to do for a key the two
+// meet later: 4 bits, 40 rows 39.0 and 40.9, 64 rows 47.1 and 41.0; dimension 64,
+// 48 rows 30.7 and 34.7, 64 rows 35.0 and 34.8. fp16: 32 rows 43.2 and 46.8, 40
+// rows 52.8 and 46.9; 4 bits 40 rows 41.3 and 46.6, 64 rows 51.4 and 47.1.
 constexpr int kManyRows = 40;
 
 // How the work is divided (one sequence at least): what runs at once on the SMs,
@@ -91,7 +93,7 @@ size_t lay_out(const nnrcu_kv_cache& c, const nnrcu_kv_attention_desc& d, Args* 
 // out, four channels a lane. A lane
 // holds one segment's share in the result, so that the segments' means are
 // loaded without waiting for one another. Starts while the attention ends, and then takes 3 to
-// 4 us, which is latency: lengths, factors, sums, one after the other. The order
+// 4 us, which is latency: lengths, shares, means, one after the other. The order
 // of the sums depends on the segments alone.
 template <int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args p) {

@@ -154,7 +154,7 @@ __device__ __forceinline__ void copy_async16(uint32_t dst, const void* src) {
 }
 
 // Blocks on an SM at once: what registers and shared memory leave room for.
-// (Three of 24 rows spill: 79 us where two take 69.)
+// (Three of 24 rows spilled: 79 us where two took 69.)
 constexpr int blocks_of_sm(int dim, bool fp32, int rows) {
   if (dim > 128) return 2;
   if (rows == 24) return 2;
@@ -331,11 +331,13 @@ __device__ __forceinline__ void store_y(const Args& p, long long at, float v) {
 // so that the codes are the 16-row operands and few query rows cost few
 // registers and little softmax; the weights change places between lanes by
 // one 8x8 transposition for each 8 keys.
-// 8 rows over 8 bits (32 sequences of 8192, 8 heads): 353 MB in 67 us, 5.3 TB/s,
-// bound by the cache's way from HBM with 16 warps on an SM. 24 rows over 4 bits
-// (7 sequences, 20001 of 30000 visible, scales of 32 channels): 66 us, bound by
-// the warps' instructions (some 1340 a tile) and latencies, with 8 warps on an
-// SM, for which the registers suffice.
+// 8 rows over 8 bits (32 sequences of 8192, 8 heads, bf16): 353 MB in 67 us,
+// 5.3 TB/s, bound by the cache's way from HBM with 16 warps on an SM (fp16, whose
+// weights have two parts: 70 us). 24 rows over 4 bits (7 sequences, 20001 of
+// 30000 visible, scales of 32 channels): the whole call 60 us in bf16 and 70 in
+// fp16, where 28.4 M warp instructions, some 1600 a tile, take less than half of
+// the issue slots: 8 warps on an SM, for which the registers suffice, do not hide
+// their latencies.
 template <int PARTS, int WPARTS, int BITS, bool GROUPED, int DP, bool EXACT, int NT>
 __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, WPARTS, BITS, GROUPED, DP, EXACT, NT>::kBlocks)
     attend_kernel(const __grid_constant__ Args p, const bool own) {
@@ -869,7 +871,8 @@ int launch(const Args& p, bool own, cudaStream_t st) {
 
 // Query rows of a block: as few blocks of up to 24 rows as there can be, since
 // each reads the keys again, and of these the smallest. 7 x 3 rows over 20000
-// 4-bit tokens: one block of 24 69 us, two of 16 75 us. Past 128 channels 8 are
+// 4-bit tokens: one block of 24 60 us in bf16 and 70 in fp16, two of 16 71 and
+// 86. Past 128 channels 8 are
 // what registers hold with two blocks on an SM: 12 rows over 32 sequences of
 // 4096, dimension 256, two blocks of 8 177 us, one of 16 256 us; 4-bit groups of
 // 32, 16 rows, 103 and 156 us; fp32 38 and 46 us.

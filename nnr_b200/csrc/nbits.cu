@@ -247,9 +247,10 @@ struct Cfg {
 // codes of a span, and its scales, through a ring of cp.async stages that runs
 // on across the items; nobody else reads them, so nothing waits for another.
 // On the device: 1x4096x4096 5.5 us, 1x16384x4096 13.5 us (2.6 TB/s of codes
-// and scales), 16x14336x4096 17.6 us. What bounds it is the warps' instructions
-// and their latencies, some 115 a tile and span of which 60 are unpacking and
-// products, with 16 to 24 warps on an SM; bytes on their way suffice.
+// and scales), 16x14336x4096 17.6 us. Its instructions, some 115 a tile and span
+// of which 60 are unpacking and products, take half of the issue slots at most
+// (1x14336x4096: IPC 2.2, 16x14336x4096: 1.6); what is left are latencies with 16
+// to 24 warps on an SM, and ends where some blocks have an item less than others.
 template <typename T, bool ZERO, int BLOCK, int RT, int TT, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, Cfg<T, ZERO, BLOCK, RT, TT, WARPS>::kBlocks)
     nbits_kernel(const __grid_constant__ NbitsArgs p, const Unpack<typename Traits<T>::type> operand) {
@@ -542,7 +543,8 @@ int launch(const NbitsArgs& p, cudaStream_t st) {
 // along again: two where every SM has work that way (1x16384x4096: 14.2 us and
 // 15.8 with one; 16x14336x4096: 18.1 and 22.0). fp32 activations cost more to take
 // apart than their codes to read, so there two are taken as soon as one a block
-// leaves SMs with two blocks to do (5x4100x2077: 8.0 us and 8.4). Where one
+// leaves SMs with two blocks to do (8x2560x8192: 16.2 us and 18.5, 16x2400x4096:
+// 14.3 and 20.5, 40x3000x3000: 20.5 and 30.7; single rows are the same). Where one
 // tile a block leaves SMs without work, those that have some get twice the
 // warps, so that twice the bytes are on their way (1x2048x4096: 4.2 us and 4.9,
 // 16x2048x8192: 7.6 and 9.2).

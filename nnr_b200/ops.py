@@ -521,7 +521,9 @@ class _Fixed:
 
 class _Plans:
     """What an operator has checked and worked out for calls with given sizes,
-    strides and types: the answer to make(*key), for the last keys seen."""
+    strides and types: the answer to make(*key), for the last keys seen. (Cache
+    attention's key holds max_len: a loop that passes each step's own length has
+    each step planned anew, one that passes a bound on all steps has not.)"""
 
     def __init__(self, make):
         self.make, self.known = make, {}
@@ -701,7 +703,11 @@ class KVAttention(_Fixed):
     """Causal attention of each sequence's newest tokens over a KVCache
     (nnrcu_kv_attention_run). scale: of the logits, 1 / sqrt(head_dim) by
     default; window: how many positions up to its own a query sees, 0 for all.
-    Both may be set anew between calls."""
+    Both may be set anew between calls.
+
+    Logits, weights' sums and results before rounding are fp32. As operands of the
+    second product, softmax weights (times their values' scales) keep 22 bits,
+    those of bf16 tensors 11; fp32 queries keep 22 bits."""
     _fixed = frozenset(("cache", "q_heads"))
 
     def __init__(self, cache: KVCache, q_heads: int, scale: Optional[float] = None, window: int = 0):
