@@ -37,13 +37,14 @@ int check(const nnrcu_kv_cache* c, const nnrcu_kv_attention_desc* d, bool buffer
 }
 
 // Rows of a key/value head from which the blocks of 128 are worth their fixed
-// cost. A prefix of 16384 keys, 8 heads, few against many (us), bf16: 8 bits and
+// cost, and as many as take the kernel for few rows two blocks, or three. A
+// prefix of 16384 keys, 8 heads, few against many (us), bf16: 8 bits and
 // dimension 128, 32 rows 40.8 and 41.1, 40 rows 50.5 and 41.4; 16 sequences of
 // 8192, 32 rows 59 and 68, 40 rows 74 and 68. With less to do for a key the two
-// meet later: 4 bits, 40 rows 39.0 and 40.9, 64 rows 47.1 and 41.0; dimension 64,
+// meet later: 4 bits, 48 rows 39.7 and 40.9, 64 rows 47.1 and 41.0; dimension 64,
 // 48 rows 30.7 and 34.7, 64 rows 35.0 and 34.8. fp16: 32 rows 43.2 and 46.8, 40
-// rows 52.8 and 46.9; 4 bits 40 rows 41.3 and 46.6, 64 rows 51.4 and 47.1.
-constexpr int kManyRows = 40;
+// rows 52.8 and 46.9; 4 bits 48 rows 43.0 and 46.8, 64 rows 51.4 and 47.1.
+constexpr int many_rows(int bits, int dim) { return bits == 8 && dim == 128 ? 40 : 56; }
 
 // How the work is divided (one sequence at least): what runs at once on the SMs,
 // or a block for each quad of keys where those are fewer.
@@ -55,7 +56,7 @@ void divide(const nnrcu_kv_cache& c, const nnrcu_kv_attention_desc& d, Args* p) 
                     (c.head_dim == 64 || c.head_dim == 128);
   auto part = [&](long long rows, long long sequences, int keys) {
     Args::Part w{};
-    w.rows = many && rows >= kManyRows ? 128 : attn::rows_of_block(rows, c.head_dim);
+    w.rows = many && rows >= many_rows(c.bits, c.head_dim) ? 128 : attn::rows_of_block(rows, c.head_dim);
     w.blocks = (int)((rows + w.rows - 1) / w.rows);
     w.units = w.blocks * c.heads;
     const long long quads = std::max(1LL, ((long long)keys + attn::kQuad - 1) / attn::kQuad);
