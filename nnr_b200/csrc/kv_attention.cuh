@@ -872,10 +872,9 @@ int launch(const Args& p, bool own, cudaStream_t st) {
 // Query rows of a block: as few blocks of up to 24 rows as there can be, since
 // each reads the keys again, and of these the smallest. 7 x 3 rows over 20000
 // 4-bit tokens: one block of 24 60 us in bf16 and 70 in fp16, two of 16 71 and
-// 86. Past 128 channels 8 are
-// what registers hold with two blocks on an SM: 12 rows over 32 sequences of
-// 4096, dimension 256, two blocks of 8 177 us, one of 16 256 us; 4-bit groups of
-// 32, 16 rows, 103 and 156 us; fp32 38 and 46 us.
+// 86. Past 128 channels 8 are what registers hold with two blocks on an SM: 12
+// rows over 32 sequences of 4096, dimension 256, two blocks of 8 177 us, one of
+// 16 256 us; 4-bit groups of 32, 16 rows, 103 and 156 us; fp32 38 and 46 us.
 inline int rows_of_block(long long rows, int dim) {
   const long long most = dim > 128 ? 8 : 24, blocks = (rows + most - 1) / most;
   return (int)(((rows + blocks - 1) / blocks + 7) / 8 * 8);

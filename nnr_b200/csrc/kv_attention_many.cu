@@ -15,11 +15,11 @@
 // another; keys and values are made fp16 in one buffer each, since they are
 // wanted at different times. A tile is 1048 cycles of products
 // (dim 128); the softmax warps keep theirs near that by working on pairs
-// (packed fp32) and in loops short enough for the instruction cache, reading S
-// twice rather than holding 128 logits. With its chain from the codes through S,
-// the weights and O a tile takes some 4000 cycles, of which the softmax passes
-// are half; the start, with q and the first tiles, and the end, with the
-// segments' sums, take some 15000 together. 128 rows of each of 8 heads over a
+// (packed fp32), 64 logits a thread, in code short enough for the instruction
+// cache. With its chain from the codes through S, the weights and O a tile takes
+// some 4000 cycles, of which the softmax passes are half; the start, with q and
+// the first tiles, and the end, with the segments' means, take some 15000
+// together. 128 rows of each of 8 heads over a
 // prefix of 16384 (8 bits, dim 128, bf16), the whole call: 47 us, and 84 with the
 // kernel for few rows; 256 rows: 67 us, in fp16 with its second product 78.
 #include "kv_attention.cuh"
