@@ -176,6 +176,9 @@ struct Cfg {
   static constexpr int kScaleBytes = kKeys * kGroups * 4;
   static constexpr int kSlot = kCodeBytes + kScaleBytes;  // keys or values of a tile
   static constexpr int kSlots = 3;
+  // The products of 32 channels are summed apart: for each group's scale, and of
+  // fp32 queries since the tensor cores cut off where an addition would round.
+  static constexpr bool kApart = GROUPED || PARTS == 2;
   static constexpr bool kQShared = PARTS * NT * DP > 512;  // q's operands in shared memory, not in registers
   static constexpr int kQBytes = kQShared ? PARTS * DP * kRows * 2 : 0;
   static constexpr int kWarpBytes = kSlots * kSlot;
@@ -571,7 +574,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, WPARTS, BITS, GROUPED,
             ldsm4<false>(w, k_s + C::place(i * 16 + (lane >> 4) * 8 + (lane & 7), c + ((lane >> 3) & 1)));
 #pragma unroll
             for (int cc = 0; cc < 2; ++cc) {
-              if (GROUPED && (BITS == 4 || cc == 0))
+              if (C::kApart && (BITS == 4 || cc == 0))
 #pragma unroll
                 for (int n = 0; n < NT; ++n) part[n][0] = part[n][1] = part[n][2] = part[n][3] = 0.f;
               const uint32_t x0 = BITS == 8 ? w[cc] ^ codes.sign : w[cc];
@@ -592,7 +595,7 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, WPARTS, BITS, GROUPED,
                       b = q_shared[((j * NT + n) * (DP / 16) + step) * 32 + lane];
                     else
                       b = make_uint2(qf[j][n][step][0], qf[j][n][step][1]);
-                    mma(GROUPED ? part[n] : s[i][n], a, b.x, b.y);
+                    mma(C::kApart ? part[n] : s[i][n], a, b.x, b.y);
                   }
               }
               if constexpr (GROUPED) {  // 8 bits: two chunks are a group; 4 bits: one is
@@ -606,6 +609,12 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, WPARTS, BITS, GROUPED,
                     s[i][n][2] = fmaf(part[n][2], f1, s[i][n][2]), s[i][n][3] = fmaf(part[n][3], f1, s[i][n][3]);
                   }
                 }
+              } else if constexpr (C::kApart) {
+                if (BITS == 4 || cc == 1)
+#pragma unroll
+                  for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[i][n][e] += part[n][e];
               }
             }
           }
@@ -767,9 +776,16 @@ __global__ void __launch_bounds__(kWarps * 32, Cfg<PARTS, WPARTS, BITS, GROUPED,
                                        BITS == 8 ? codes.from8(x1, 0x4240) : codes.from4(x1 >> (8 * st)),
                                        BITS == 8 ? codes.from8(x1, 0x4341) : codes.from4(x1 >> (8 * st + 4))};
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int n = 0; n < NT; ++n) {
+                  float(&sum)[4] = o[(c + cc) * C::kSteps + st][n];
+                  float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                  for (int j = 0; j < WPARTS; ++j) mma(o[(c + cc) * C::kSteps + st][n], a, b[n][j][0], b[n][j][1]);
+                  for (int j = 0; j < WPARTS; ++j) mma(PARTS == 2 ? part : sum, a, b[n][j][0], b[n][j][1]);
+                  if constexpr (PARTS == 2) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sum[e] += part[e];
+                  }
+                }
               }
             }
           }

@@ -352,3 +352,22 @@ def test_attention_in_fp16_is_off_by_its_rounding_only(kind, batch, longest, pre
     if longest == 1 and not prefix:
         v = values(cache, "v")[table[:, 0].long(), 0].half()
         assert torch.equal(got[:, 0], v.repeat_interleave(4, 1))
+
+
+@pytest.mark.parametrize("kind,batch,longest", [((8, 0, 128, 8, 64), 8, 8192), ((8, 0, 128, 5, 48), 1, 30000),
+                                                ((8, 0, 256, 2, 48), 3, 200), ((4, 0, 64, 8, 16), 8, 9000),
+                                                ((4, 32, 128, 4, 16), 8, 6000)])
+@pytest.mark.parametrize("seed", [1, 2, 3])
+def test_attention_in_fp32_is_off_by_few_roundings(kind, batch, longest, seed):
+    """In the norm of the output. A logit of up to 16 has steps of 2^-20 (half of
+    one is 2^-21 of its p), exp2 is off by 2^-22 and so are operands of 22 bits:
+    together less than 2^-20, if the sums of both products add nothing."""
+    bits, group, dim, heads, page = kind
+    per = -(-longest // page)
+    cache = filled(kind, batch * per, seed)
+    table, _ = layout(cache, batch, longest, 0, seed)
+    lens = torch.full((batch,), longest, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, 1, heads, dim, generator=generator(seed), device="cuda") * 1.25
+    got = ops.KVAttention(cache, heads).exec(q, table, lens).double()
+    want, _ = attention_ref(cache, q, table, lens, None, 0, 0, dim ** -0.5, "f32")
+    assert (got - want).norm() <= want.norm() * 2.0 ** -20
